@@ -383,6 +383,78 @@ int iomb_sdpa_scale_mask_softmax(const iomb_sdpa_stages* stages, int keep_scores
  */
 int iomb_sdpa_canonicalize_output(const iomb_view* out, void* stream);
 
+/*
+ * Causal attention over packed prompts: out[t, h*D + d] = sum_j w_j v[h/G, j, d] with w the
+ * softmax of scale * q[h, t].k[h/G, j] over the rows j of t's own sequence up to and with t,
+ * G = Hq / Hkv. q is [Hq, T, D], k and v [Hkv, T, D], out [T, Hq*D] (the merged layout of
+ * iomb_sdpa_canonicalize_output), one leaf: BF16 or F16. `offsets` is a device array of
+ * sequences + 1 ascending rows; sequence s holds the rows offsets[s] .. offsets[s+1]-1, which
+ * may be none. Rows outside every sequence are neither read nor written. `status` (device
+ * word) becomes 0, or 1 when the offsets descend or pass T: then nothing is written.
+ * Scores, the softmax's maximum and sum and the weighted sum are binary32; the weights are
+ * rounded to the leaf once, before they meet v, and the result once, when it is stored. Special rows as in
+ * iomb_sdpa_softmax: a NaN among a row's scores, or only -inf, makes the row the quiet NaN,
+ * +inf scores share the weight; stored -0 and NaN are canonical. What masked places hold has
+ * no influence. D up to 256; multiples of 16 up to 128 run on the tensor cores. `scale` is positive and
+ * finite (1/sqrtf(D) usually). The output overlaps no input.
+ * No counterpart in the reference, whose sdpa takes one sequence (the caller's loop over
+ * sequences gives the same rows).
+ */
+int iomb_sdpa_packed(const iomb_view* q, const iomb_view* k, const iomb_view* v, const iomb_view* out,
+                     const uint32_t* offsets, uint32_t sequences, float scale, uint32_t* status,
+                     void* stream);
+
+/*
+ * Attention of drafted token trees over KV caches: q is [B, Hq, N, D] (N up to 256 nodes of one
+ * tree per sequence), k and v are caches [B, Hkv, C, D], out [B, N, Hq*D]; leaves, arithmetic
+ * and special rows as iomb_sdpa_packed. Device arrays: lengths[b] is the number of cache rows
+ * before the tree, whose node i lies at cache row lengths[b] + i (iomb_cache_append_batched at
+ * `lengths` puts it there); parents[b*N + i] < i is node i's parent or -1 for a root (NULL:
+ * every tree is a chain); counts[b] <= N is the number of nodes in use (NULL: N). Node i sees
+ * the rows before the tree, its ancestors and itself. N = 1 is the single-token decode. Output
+ * rows at or beyond counts[b] keep their bytes. `status` becomes 0, or 1 when a sequence does
+ * not fit (lengths[b] + counts[b] > C or counts[b] > N: it is skipped) or a parent does not
+ * lie before its node or is below -1 (the node then counts as a root).
+ * `workspace` holds iomb_sdpa_tree_workspace_bytes bytes of device memory, 32-byte aligned:
+ * long caches are cut into ranges whose partial sums meet there. Its contents need no set-up
+ * and mean nothing after the call; two calls that may overlap on the GPU use two workspaces.
+ * No counterpart in the reference.
+ */
+int iomb_sdpa_tree_workspace_bytes(const iomb_view* q, const iomb_view* k, uint64_t* bytes);
+int iomb_sdpa_tree(const iomb_view* q, const iomb_view* k, const iomb_view* v, const iomb_view* out,
+                   const uint32_t* lengths, const int32_t* parents, const uint32_t* counts, float scale,
+                   void* workspace, uint64_t workspace_bytes, uint32_t* status, void* stream);
+
+/*
+ * Keeps the accepted rows of a tree: cache[b, ..., lengths[b] + j, d] =
+ * cache[b, ..., lengths[b] + accepted[b*width + j], d] for j < counts[b], in place (raw bits),
+ * on the caches k and v [B, ..., C, D] of one shape (v may be NULL: one cache). The device
+ * array `accepted` is [B, width]; a sequence's path ascends strictly below width, as a walk
+ * from a root does. No other row changes. `status` becomes 0, or 1 when some path does not
+ * ascend, reaches width or the end of the cache, or counts[b] > width: that b is skipped.
+ * Byte-multiple leaves. The planes of a view are distinct, and k and v do not overlap.
+ * No counterpart in the reference.
+ */
+int iomb_cache_compact(const iomb_view* k, const iomb_view* v, const uint32_t* lengths,
+                       const uint32_t* accepted, uint32_t width, const uint32_t* counts,
+                       uint32_t* status, void* stream);
+
+/*
+ * Scores of given tokens: logprob[..., 0, r] = log softmax(logits[..., r, :])[tokens[..., 0, r]],
+ * entropy[..., 0, r] = -sum p log p of the row (NULL: not wanted), and the K <= 32 best tokens
+ * of the row with their log probabilities, top_tokens and top_logprobs [..., R, K] (NULL, both:
+ * not wanted). Best is the larger logit, equal ones by the lower token, -0 equal to +0, NaN
+ * above everything. logits [..., R, V]: BF16, F16 or F32; tokens [..., 1, R]: I32, U32, I64 or
+ * U64; results F32, top_tokens U32 or I32. Sums are binary32. -inf logits (tokens ruled out)
+ * have probability zero; a row that holds NaN, +inf or nothing but -inf has NaN results.
+ * `status` (device word) becomes 0, or 1 when a token is negative or >= V: its log
+ * probability keeps its bytes. Results overlap no other operand. No counterpart in the
+ * reference, whose selector reads the logits on the host (src/token_selection.cpp).
+ */
+int iomb_token_logprobs(const iomb_view* logits, const iomb_view* tokens, const iomb_view* logprob,
+                        const iomb_view* entropy, const iomb_view* top_logprobs,
+                        const iomb_view* top_tokens, uint32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -83,6 +83,16 @@ PROTOTYPES = {
     "iomb_sdpa_scale_mask_softmax": (ctypes.c_int, [ctypes.POINTER(IombSdpaStages), ctypes.c_int,
                                                     ctypes.c_void_p]),
     "iomb_sdpa_canonicalize_output": (ctypes.c_int, [_VIEW, ctypes.c_void_p]),
+    "iomb_sdpa_packed": (ctypes.c_int, [_VIEW, _VIEW, _VIEW, _VIEW, ctypes.c_void_p, ctypes.c_uint32,
+                                        ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p]),
+    "iomb_sdpa_tree_workspace_bytes": (ctypes.c_int, [_VIEW, _VIEW, _U64P]),
+    "iomb_sdpa_tree": (ctypes.c_int, [_VIEW, _VIEW, _VIEW, _VIEW, ctypes.c_void_p, ctypes.c_void_p,
+                                      ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p, ctypes.c_uint64,
+                                      ctypes.c_void_p, ctypes.c_void_p]),
+    "iomb_cache_compact": (ctypes.c_int, [_VIEW, _VIEW, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32,
+                                          ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "iomb_token_logprobs": (ctypes.c_int, [_VIEW, _VIEW, _VIEW, _VIEW, _VIEW, _VIEW, ctypes.c_void_p,
+                                           ctypes.c_void_p]),
 }
 
 _library = None

@@ -231,6 +231,100 @@ cache_append_kernel(const AppendParams p) {
     }
 }
 
+// ---- cache compact ---------------------------------------------------------------
+
+struct CompactParams {
+    Operand cache[2];           // K and V (or one cache)
+    Leading leading;            // not collapsed: the first axis is the batch
+    RowGeometry row;
+    uint32_t caches;
+    uint64_t planes;            // logical planes of one cache
+    uint64_t planes_per_batch;
+    uint64_t cache_rows;        // C
+    uint32_t batch, width;
+    const uint32_t* lengths;
+    const uint32_t* accepted;   // [batch, width]
+    const uint32_t* counts;
+    uint32_t* status;
+};
+
+// Whether accepted[j] of a sequence that keeps `count` rows of `length` is in order: paths
+// ascend, and everything lies inside the tree and the cache.
+__device__ __forceinline__ bool path_step_ok(const CompactParams& p, uint32_t b, uint64_t length,
+                                             uint32_t count, uint32_t j) {
+    const uint32_t* path = p.accepted + static_cast<uint64_t>(b) * p.width;
+    const uint32_t at = path[j];
+    return at < p.width && length + at < p.cache_rows && (j == 0 || path[j - 1] < at);
+}
+
+// One warp moves one plane's accepted rows. Items are (tile column, row, 16-byte vector) with
+// the row ascending inside a column: accepted[j] >= j and ascending, so a row is written only
+// after every row that still has to be read from it (itself and those before it in the path)
+// was read, whether the two lie in one chunk (all loads of a chunk come before its stores) or
+// in two. Latency bound: a call moves a few KB per plane in two dependent round trips (the
+// path, the rows), with four items per lane in flight.
+constexpr uint32_t kCompactItems = 4;
+
+__global__ void __launch_bounds__(kRowThreads)
+cache_compact_kernel(const CompactParams p) {
+    // The last block checks every path and reports.
+    if (blockIdx.x == gridDim.x - 1) {
+        bool bad = false;
+        const uint64_t all = static_cast<uint64_t>(p.batch) * p.width;
+        for (uint64_t i = threadIdx.x; i < all; i += kRowThreads) {
+            const uint32_t b = static_cast<uint32_t>(i / p.width), j = static_cast<uint32_t>(i % p.width);
+            const uint32_t count = p.counts[b];
+            bad = bad || count > p.width || (j < count && !path_step_ok(p, b, p.lengths[b], count, j));
+        }
+        const int any = __syncthreads_or(bad ? 1 : 0);
+        if (threadIdx.x == 0) *p.status = any ? 1u : 0u;
+        return;
+    }
+    const uint32_t lane = threadIdx.x & 31u;
+    const uint64_t unit = static_cast<uint64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5);
+    if (unit >= p.planes * p.caches) return;
+    const uint32_t which = static_cast<uint32_t>(unit / p.planes);
+    const uint64_t index = unit % p.planes;
+    const uint32_t b = static_cast<uint32_t>(index / p.planes_per_batch);
+    const uint32_t count = p.counts[b];
+    const uint64_t length = p.lengths[b];
+    bool ok = count <= p.width;
+    for (uint32_t j = lane; j < count && ok; j += 32) ok = path_step_ok(p, b, length, count, j);
+    if (!__all_sync(0xffffffffu, ok) || count == 0) return;
+    const uint32_t* path = p.accepted + static_cast<uint64_t>(b) * p.width;
+    const Operand& cache = p.cache[which];
+    const uint64_t plane = operand_plane(cache, p.leading, index);
+    const uint32_t elem = p.row.elem, per_vector = 16 / elem;
+    const uint32_t column_items = count * elem;                  // vectors of one tile column
+    const uint64_t items = static_cast<uint64_t>(column_items) * p.row.tile_cols;
+    for (uint64_t first = 0; first < items; first += 32 * kCompactItems) {
+        uint4 value[kCompactItems];
+        unsigned char* dst[kCompactItems];
+        uint32_t valid[kCompactItems];
+#pragma unroll
+        for (uint32_t u = 0; u < kCompactItems; ++u) {
+            const uint64_t item = first + u * 32 + lane;
+            valid[u] = 0;
+            if (item >= items) continue;
+            const uint32_t tc = static_cast<uint32_t>(item / column_items);
+            const uint32_t rest = static_cast<uint32_t>(item % column_items);
+            const uint32_t j = rest / elem, cv = rest % elem;
+            const uint32_t from = path[j];
+            const uint32_t col = tc * kTile + cv * per_vector;
+            if (from == j || col >= p.row.cols) continue;
+            valid[u] = min(per_vector, p.row.cols - col);
+            value[u] = load_u4(piece_address(cache, plane, length + from, tc, elem) + cv * 16);
+            dst[u] = piece_address(cache, plane, length + j, tc, elem) + cv * 16;
+        }
+        __syncwarp();
+#pragma unroll
+        for (uint32_t u = 0; u < kCompactItems; ++u) {
+            if (valid[u] != 0) store_row_vector(dst[u], value[u], valid[u], per_vector, elem);
+        }
+        __syncwarp();
+    }
+}
+
 // ---- host dispatch ---------------------------------------------------------------
 
 static RowGeometry row_geometry(const ViewFacts& f) {
@@ -467,4 +561,80 @@ extern "C" int iomb_cache_append_batched(const iomb_view* source, const iomb_vie
         return iomb::fail(IOMB_ERR_INVALID_ARGUMENT, "cache_append_batched: positions is null");
     }
     return iomb::append_dispatch(source, destination, 0, positions, status, stream);
+}
+
+extern "C" int iomb_cache_compact(const iomb_view* k, const iomb_view* v, const uint32_t* lengths,
+                                  const uint32_t* accepted, uint32_t width, const uint32_t* counts,
+                                  uint32_t* status, void* stream) {
+    using namespace iomb;
+    ViewFacts fk{}, fv{};
+    int rc = check_view(k, "cache_compact k", &fk);
+    if (rc == IOMB_OK && v != nullptr) rc = check_view(v, "cache_compact v", &fv);
+    if (rc != IOMB_OK) return rc;
+    if (k->rank < 3) return fail(IOMB_ERR_INVALID_ARGUMENT, "cache_compact requires ranks of three through eight");
+    if (v != nullptr) {
+        bool same = k->rank == v->rank && k->dtype == v->dtype;
+        for (uint32_t i = 0; i < k->rank && same; ++i) same = k->dims[i] == v->dims[i];
+        if (!same) return fail(IOMB_ERR_INVALID_ARGUMENT, "cache_compact: k and v shapes or encodings differ");
+        if (storage_overlaps(*k, fk, *v, fv)) {
+            return fail(IOMB_ERR_INVALID_ARGUMENT, "cache_compact: k and v storage overlap");
+        }
+    }
+    for (const iomb_view* view : {k, v}) {
+        // Rows move in place, so two indices must not name one plane.
+        if (view == nullptr) continue;
+        uint64_t pairs[kMaxLead][2];
+        uint32_t n = 0;
+        for (uint32_t axis = 0; axis + 2 < view->rank; ++axis) {
+            if (view->dims[axis] == 1) continue;
+            uint32_t at = n++;
+            while (at > 0 && pairs[at - 1][0] > view->plane_strides[axis]) {
+                pairs[at][0] = pairs[at - 1][0];
+                pairs[at][1] = pairs[at - 1][1];
+                --at;
+            }
+            pairs[at][0] = view->plane_strides[axis];
+            pairs[at][1] = view->dims[axis];
+        }
+        uint64_t reach = 0;     // furthest plane the axes with smaller strides get to
+        for (uint32_t i = 0; i < n; ++i) {
+            if (pairs[i][0] <= reach) {
+                return fail(IOMB_ERR_INVALID_ARGUMENT, "cache_compact: planes of the cache overlap");
+            }
+            reach += pairs[i][0] * (pairs[i][1] - 1);
+        }
+    }
+    for (const void* address : {static_cast<const void*>(lengths), static_cast<const void*>(accepted),
+                                static_cast<const void*>(counts), static_cast<const void*>(status)}) {
+        if (address == nullptr || reinterpret_cast<uintptr_t>(address) % 4 != 0) {
+            return fail(IOMB_ERR_INVALID_ARGUMENT,
+                        "cache_compact: lengths, accepted, counts and status are device arrays of words");
+        }
+    }
+    if (width == 0) return fail(IOMB_ERR_INVALID_ARGUMENT, "cache_compact: width must be nonzero");
+    if (fk.bytes == 0) return fail(IOMB_ERR_UNSUPPORTED, "cache_compact: sub-byte leaves are not implemented");
+    if (width > (1u << 20) || k->dims[0] > 0xFFFFFFFFull || fk.rows > 0xFFFFFFFFull || fk.cols > 0xFFFFFFFFull) {
+        return fail(IOMB_ERR_UNSUPPORTED, "cache_compact: an extent exceeds the kernel limit");
+    }
+    CompactParams p{};
+    p.leading.count = fk.leading;
+    p.leading.planes = fk.planes;
+    for (uint32_t axis = 0; axis < kMaxLead; ++axis) p.leading.dims[axis] = axis < fk.leading ? k->dims[axis] : 1;
+    p.cache[0] = make_operand(*k, fk, k->plane_strides, p.leading, false, false);
+    if (v != nullptr) p.cache[1] = make_operand(*v, fv, v->plane_strides, p.leading, false, false);
+    p.caches = v != nullptr ? 2 : 1;
+    p.row = row_geometry(fk);
+    p.planes = fk.planes;
+    p.planes_per_batch = fk.planes / k->dims[0];
+    p.cache_rows = fk.rows;
+    p.batch = static_cast<uint32_t>(k->dims[0]);
+    p.width = width;
+    p.lengths = lengths;
+    p.accepted = accepted;
+    p.counts = counts;
+    p.status = status;
+    const uint64_t blocks = (p.planes * p.caches + kRowWarps - 1) / kRowWarps + 1;
+    if (blocks > 0x7FFFFFFFull) return fail(IOMB_ERR_UNSUPPORTED, "cache_compact: too many planes for one launch");
+    cache_compact_kernel<<<static_cast<unsigned>(blocks), kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    return check_launch("cache_compact launch");
 }

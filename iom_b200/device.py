@@ -1025,3 +1025,92 @@ class B200Queue:
         return self._submit(
             lambda stream: self._lib.iomb_sdpa_canonicalize_output(ctypes.byref(view), stream),
             (out.owner,))
+
+    # -- generation over caches (extensions) -----------------------------------
+    # Small index arrays are device addresses of uint32 words (int32 for parents), as in
+    # cache_append_batched; `status` is a device word that becomes 0, or 1 when the arrays'
+    # values do not fit. They are read when the operation runs.
+    def _operands(self, what: str, *views):
+        """The ABI snapshots of an operation's views (None stays None)."""
+        for view in views:
+            if view is not None:
+                self._check_view(view, what)
+        return [None if view is None else ctypes.byref(view.as_abi()) for view in views]
+
+    def sdpa_packed(self, q: TensorView, k: TensorView, v: TensorView, out: TensorView,
+                    offsets: int, sequences: int, status: int, scale: Optional[float] = None) -> int:
+        """Extension: causal attention over packed prompts. q [Hq, T, D], k and v [Hkv, T, D],
+        out [T, Hq*D], BF16 or F16; `offsets` holds sequences + 1 ascending row borders. `scale`
+        None is 1/sqrt(D). See iomb_sdpa_packed."""
+        try:
+            a, b, c, d = self._operands("sdpa_packed", q, k, v, out)
+            if not 0 <= sequences < 1 << 32:
+                raise ValueError("sdpa_packed: the number of sequences is out of range")
+            if scale is None:
+                scale = q.spec.shape[-1] ** -0.5
+        except BaseException as error:
+            return _exception_to_oid(error)
+        return self._submit(
+            lambda stream: self._lib.iomb_sdpa_packed(a, b, c, d, offsets, sequences, scale, status, stream),
+            (q.owner, k.owner, v.owner, out.owner))
+
+    def sdpa_tree_workspace_requirements(self, q: TensorView, k: TensorView) -> WorkspaceRequirements:
+        a, b = self._operands("sdpa_tree", q, k)
+        nbytes = ctypes.c_uint64()
+        status = self._lib.iomb_sdpa_tree_workspace_bytes(a, b, ctypes.byref(nbytes))
+        if status != 0:
+            raise _status_to_exception(status)
+        return WorkspaceRequirements(nbytes.value, 32 if nbytes.value else 1)
+
+    def sdpa_tree(self, q: TensorView, k: TensorView, v: TensorView, out: TensorView,
+                  lengths: int, parents: int, counts: int, status: int,
+                  workspace: Optional[RawWorkspaceView] = None, scale: Optional[float] = None) -> int:
+        """Extension: attention of drafted token trees over KV caches; one node per sequence is
+        the single-token decode. q [B, Hq, N, D], k and v [B, Hkv, C, D], out [B, N, Hq*D];
+        `parents` 0 makes every tree a chain, `counts` 0 means N nodes each. See iomb_sdpa_tree."""
+        try:
+            a, b, c, d = self._operands("sdpa_tree", q, k, v, out)
+            address, nbytes, owner = 0, 0, None
+            if workspace is not None and not workspace.empty():
+                if not self._device.owns_workspace(workspace.owner):
+                    raise ValueError("sdpa_tree requires a live workspace of this device")
+                address, nbytes, owner = workspace.address(), workspace.byte_size(), workspace.owner
+            if scale is None:
+                scale = q.spec.shape[-1] ** -0.5
+        except BaseException as error:
+            return _exception_to_oid(error)
+        return self._submit(
+            lambda stream: self._lib.iomb_sdpa_tree(a, b, c, d, lengths, parents or None, counts or None, scale,
+                                                    address, nbytes, status, stream),
+            (q.owner, k.owner, v.owner, out.owner, owner))
+
+    def cache_compact(self, k: TensorView, v: Optional[TensorView], lengths: int, accepted: int,
+                      width: int, counts: int, status: int) -> int:
+        """Extension: the accepted rows of every sequence's tree move to the front of it, in
+        place, in caches [B, ..., C, D]; `accepted` is [B, width], ascending. See
+        iomb_cache_compact."""
+        try:
+            a, b = self._operands("cache_compact", k, v)
+            if not 0 <= width < 1 << 32:
+                raise ValueError("cache_compact: width is out of range")
+        except BaseException as error:
+            return _exception_to_oid(error)
+        return self._submit(
+            lambda stream: self._lib.iomb_cache_compact(a, b, lengths, accepted, width, counts, status, stream),
+            (k.owner, None if v is None else v.owner))
+
+    def token_logprobs(self, logits: TensorView, tokens: TensorView, logprob: TensorView,
+                       entropy: Optional[TensorView], status: int,
+                       top_logprobs: Optional[TensorView] = None,
+                       top_tokens: Optional[TensorView] = None) -> int:
+        """Extension: log probabilities of given tokens, the rows' entropy and their best
+        tokens. logits [..., R, V], tokens, logprob and entropy [..., 1, R], top_* [..., R, K].
+        See iomb_token_logprobs."""
+        try:
+            views = (logits, tokens, logprob, entropy, top_logprobs, top_tokens)
+            a, b, c, d, e, f = self._operands("token_logprobs", *views)
+        except BaseException as error:
+            return _exception_to_oid(error)
+        return self._submit(
+            lambda stream: self._lib.iomb_token_logprobs(a, b, c, d, e, f, status, stream),
+            tuple(view.owner for view in views if view is not None))
