@@ -425,6 +425,10 @@ int iomb_sdpa_tree(const iomb_view* q, const iomb_view* k, const iomb_view* v, c
                    const uint32_t* lengths, const int32_t* parents, const uint32_t* counts, float scale,
                    void* workspace, uint64_t workspace_bytes, uint32_t* status, void* stream);
 
+/* iomb_rmsnorm_copy_timeouts for the attention kernels: CTAs in which a bounded wait gave up
+ * (never expected: their results are incomplete). Synchronous. */
+int iomb_sdpa_wait_timeouts(unsigned int* count);
+
 /*
  * Keeps the accepted rows of a tree: cache[b, ..., lengths[b] + j, d] =
  * cache[b, ..., lengths[b] + accepted[b*width + j], d] for j < counts[b], in place (raw bits),

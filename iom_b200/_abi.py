@@ -89,6 +89,7 @@ PROTOTYPES = {
     "iomb_sdpa_tree": (ctypes.c_int, [_VIEW, _VIEW, _VIEW, _VIEW, ctypes.c_void_p, ctypes.c_void_p,
                                       ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p, ctypes.c_uint64,
                                       ctypes.c_void_p, ctypes.c_void_p]),
+    "iomb_sdpa_wait_timeouts": (ctypes.c_int, [ctypes.POINTER(ctypes.c_uint)]),
     "iomb_cache_compact": (ctypes.c_int, [_VIEW, _VIEW, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32,
                                           ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     "iomb_token_logprobs": (ctypes.c_int, [_VIEW, _VIEW, _VIEW, _VIEW, _VIEW, _VIEW, ctypes.c_void_p,

@@ -17,7 +17,7 @@ PACKAGE_DIR = Path(__file__).resolve().parent
 CSRC = PACKAGE_DIR / "csrc"
 LIBRARY = PACKAGE_DIR / "libiom_b200.so"
 SOURCES = ["host.cu", "binary.cu", "rmsnorm.cu", "rmsnorm_long.cu", "copy.cu", "gather.cu", "sumsq.cu", "silu.cu", "rope.cu", "sdpa.cu",
-           "attention.cu", "logprobs.cu"]
+           "attention.cu", "attention_tc.cu", "logprobs.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

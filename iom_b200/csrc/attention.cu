@@ -64,6 +64,7 @@ static AttnOperand attn_operand(const iomb_view& view, const ViewFacts& f, int a
     o.plane0 = view.plane_offset;
     o.stride_b = axis_b >= 0 ? view.plane_strides[axis_b] : 0;
     o.stride_h = axis_h >= 0 ? view.plane_strides[axis_h] : 0;
+    o.planes = f.max_plane + 1;
     o.tile_rows = static_cast<uint32_t>(f.tile_rows);
     o.tile_cols = static_cast<uint32_t>(f.tile_cols);
     return o;
@@ -106,12 +107,11 @@ static int admit(const char* name, const iomb_view* q, const iomb_view* k, const
         return refuse(IOMB_ERR_INVALID_ARGUMENT, "query heads are not a multiple of the key/value heads");
     }
     if (fk.cols != fq.cols) return refuse(IOMB_ERR_INVALID_ARGUMENT, "head widths differ");
-    // (each below 2^31 here would do; the checked view arithmetic bounds the product)
     if (fq.cols > kMaxHeadWidth) return refuse(IOMB_ERR_UNSUPPORTED, "head width exceeds 256");
     if (fo.rows != fq.rows || fo.cols != hq * fq.cols) {
         return refuse(IOMB_ERR_INVALID_ARGUMENT, "out must hold one row of Hq * D per row of q");
     }
-    if (fq.rows > (1ull << 30) || fk.rows > (1ull << 30) || hq > (1ull << 20) || (lead == 1 && q->dims[0] > (1ull << 20))) {
+    if (fq.rows > kMaxAttnRows || fk.rows > kMaxAttnRows || hq > kMaxAttnExtent || (lead == 1 && q->dims[0] > kMaxAttnExtent)) {
         return refuse(IOMB_ERR_UNSUPPORTED, "an extent exceeds the kernel limit");
     }
     if (!(scale > 0.0f) || !isfinite(scale)) {
@@ -160,20 +160,13 @@ extern "C" int iomb_sdpa_packed(const iomb_view* q, const iomb_view* k, const io
     p.offsets = offsets;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool bf16 = q->dtype == IOMB_BF16;
+    if (attention_tc_takes(p)) return launch_attention_tc(p, false, bf16, nullptr, s);
     const uint64_t rows = static_cast<uint64_t>(p.rows) * p.hq;
     const unsigned grid = grid_for((rows + kRowWarpsPerCta - 1) / kRowWarpsPerCta, 8);
     if (bf16) packed_rows_kernel<LeafBf16><<<grid, kRowWarpsPerCta * 32, 0, s>>>(p);
     else packed_rows_kernel<LeafF16><<<grid, kRowWarpsPerCta * 32, 0, s>>>(p);
     return check_launch("sdpa_packed launch");
 }
-
-namespace iomb {
-static int admit_tree_shape(const AttnParams& p, uint64_t batch) {
-    if (p.rows > kMaxTreeNodes) return fail(IOMB_ERR_UNSUPPORTED, "sdpa_tree: a tree holds at most 256 nodes");
-    if (batch == 0) return fail(IOMB_ERR_INVALID_ARGUMENT, "sdpa_tree: no sequences");
-    return IOMB_OK;
-}
-}  // namespace iomb
 
 extern "C" int iomb_sdpa_tree_workspace_bytes(const iomb_view* q, const iomb_view* k, uint64_t* bytes) {
     using namespace iomb;
@@ -182,7 +175,22 @@ extern "C" int iomb_sdpa_tree_workspace_bytes(const iomb_view* q, const iomb_vie
     int rc = check_view(q, "sdpa_tree q", &fq);
     if (rc == IOMB_OK) rc = check_view(k, "sdpa_tree k", &fk);
     if (rc != IOMB_OK) return rc;
-    *bytes = 0;
+    if (q->rank != 4 || k->rank != 4 || q->dims[0] != k->dims[0] || q->dims[1] % k->dims[1] != 0 || fq.cols != fk.cols) {
+        return fail(IOMB_ERR_INVALID_ARGUMENT, "sdpa_tree: shapes must be q [B,Hq,N,D] and k [B,Hkv,C,D], Hq a multiple of Hkv");
+    }
+    if (q->dims[0] > kMaxAttnExtent || q->dims[1] > kMaxAttnExtent || fq.rows > kMaxTreeNodes || fk.rows > kMaxAttnRows
+            || fq.cols > kMaxHeadWidth) {
+        return fail(IOMB_ERR_UNSUPPORTED, "sdpa_tree: an extent exceeds the kernel limit");
+    }
+    AttnParams p{};
+    p.k = p.v = attn_operand(*k, fk, 0, 1);
+    p.hkv = static_cast<uint32_t>(k->dims[1]);
+    p.group = static_cast<uint32_t>(q->dims[1] / k->dims[1]);
+    p.width = static_cast<uint32_t>(fq.cols);
+    p.rows = static_cast<uint32_t>(fq.rows);
+    p.cache_rows = static_cast<uint32_t>(fk.rows);
+    p.batch = static_cast<uint32_t>(q->dims[0]);
+    *bytes = attention_tc_takes(p) ? attention_tc_workspace(p) : 0;
     return IOMB_OK;
 }
 
@@ -191,10 +199,9 @@ extern "C" int iomb_sdpa_tree(const iomb_view* q, const iomb_view* k, const iomb
                               void* workspace, uint64_t workspace_bytes, uint32_t* status, void* stream) {
     using namespace iomb;
     AttnParams p{};
-    int rc = admit("sdpa_tree", q, k, v, out, 1, scale, status, &p);
+    const int rc = admit("sdpa_tree", q, k, v, out, 1, scale, status, &p);
     if (rc != IOMB_OK) return rc;
-    rc = admit_tree_shape(p, q->dims[0]);
-    if (rc != IOMB_OK) return rc;
+    if (p.rows > kMaxTreeNodes) return fail(IOMB_ERR_UNSUPPORTED, "sdpa_tree: a tree holds at most 256 nodes");
     if (lengths == nullptr || !aligned4(lengths) || !aligned4(parents) || !aligned4(counts)) {
         return fail(IOMB_ERR_INVALID_ARGUMENT, "sdpa_tree: lengths, parents and counts are device arrays of words");
     }
@@ -204,8 +211,14 @@ extern "C" int iomb_sdpa_tree(const iomb_view* q, const iomb_view* k, const iomb
     p.counts = counts;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool bf16 = q->dtype == IOMB_BF16;
-    (void)workspace;
-    (void)workspace_bytes;
+    if (attention_tc_takes(p)) {
+        const uint64_t need = attention_tc_workspace(p);
+        if (need != 0 && (workspace == nullptr || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 32 != 0)) {
+            return fail(IOMB_ERR_INVALID_ARGUMENT,
+                        "sdpa_tree: the workspace is smaller than iomb_sdpa_tree_workspace_bytes or not 32-byte aligned");
+        }
+        return launch_attention_tc(p, true, bf16, workspace, s);
+    }
     const uint64_t rows = static_cast<uint64_t>(p.batch) * p.hq * p.rows;
     const unsigned grid = grid_for((rows + kRowWarpsPerCta - 1) / kRowWarpsPerCta, 8);
     if (bf16) tree_rows_kernel<LeafBf16><<<grid, kRowWarpsPerCta * 32, 0, s>>>(p);

@@ -17,12 +17,14 @@ namespace iomb {
 
 constexpr uint32_t kMaxHeadWidth = 256;     // row-at-a-time form: eight values per lane
 constexpr uint32_t kMaxTreeNodes = 256;
+constexpr uint64_t kMaxAttnRows = 1ull << 30, kMaxAttnExtent = 1ull << 20;     // tokens; heads, sequences
 constexpr uint32_t kKvBlock = 128;          // tokens per block of the tensor-core kernel
 
 // One operand [b, h, rows, columns]: its planes by two strides (0 where the axis is absent).
 struct AttnOperand {
     unsigned char* base;
     uint64_t plane0, stride_b, stride_h;
+    uint64_t planes;            // planes of the owner up to the view's last
     uint32_t tile_rows, tile_cols;
 };
 
@@ -268,7 +270,7 @@ __device__ __forceinline__ void warp_report_tree(const AttnParams& p) {
     if (lane == 0) *p.status = bad ? 1u : 0u;
 }
 
-// The tensor-core kernel (attention_tc.cu).
+// The tensor-core kernel (attention_tc.cu). The workspace is the partial sums of a tree call.
 bool attention_tc_takes(const AttnParams& p);
 uint64_t attention_tc_workspace(const AttnParams& p);
 int launch_attention_tc(const AttnParams& p, bool tree, bool bf16, void* workspace, cudaStream_t stream);

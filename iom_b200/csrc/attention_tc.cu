@@ -1,0 +1,1173 @@
+// Attention on the tensor cores: the kernel behind iomb_sdpa_packed and iomb_sdpa_tree for head
+// widths that are multiples of 16 up to 128.
+//
+// One CTA works on two tiles, A and B, of 128 score rows each. Per block of 128 tokens and tile
+//   S = Q K^T          tcgen05.mma, both operands in shared memory, S in tensor memory (FP32)
+//   P = exp2(c S - c m) softmax warpgroup of the tile: one thread per row, S read back from
+//                      tensor memory, P (16-bit) written over S
+//   O += P V           tcgen05.mma, P from tensor memory, V from shared memory, O in tensor memory
+// with the running maximum m and sum l of each row in its thread. O is rescaled only when a
+// row's maximum grows by more than 2^8 (P then stays below 2^8, far from any overflow); the sum
+// takes the unrounded exponentials. While one tile's softmax runs, the other tile's products do.
+//
+// The library's 16x16 tiles feed the matrix instructions without any re-layout: a tile row is 32
+// bytes, so a column of tiles is a K-major operand with 32-byte swizzle and K = 16 (one
+// instruction) for Q and K, and the same bytes are the MN-major operand of V. One tensor-map
+// copy per block fetches 128 tokens x D as [D/16][8 tiles][16][32 B].
+//
+// What a tile's 128 rows are:
+//   packed   `pack` heads of one key/value head x 128/pack consecutive rows, so that short
+//            sequences share a tile between heads; A and B are neighbouring row blocks
+//   tree     the (head, node) pairs of one key/value head. Up to 128 pairs: both tiles hold the
+//            same rows and take alternate token blocks, joined at the end. More: A and B hold
+//            128 pairs each and share the token blocks
+// The tree call cuts the token blocks of all sequences and heads into equal ranges, one per CTA.
+// A row whose blocks lie in several ranges leaves partial (m, l, O) in the workspace and a second
+// kernel joins them, in the order of the ranges.
+//
+// Special rows: a row with a result that is not finite (NaN or infinities among its operands,
+// but also garbage under the mask, which the matrix instruction multiplies by zero) is computed
+// again by attend_row, which reads visible tokens only.
+//
+// Warps: 0-3 softmax of A, 4-7 softmax of B, 8 issues the matrix instructions, 9 the copies (10
+// and 11 fill their warpgroup, which hands registers to the softmax: 2 x 128 x 208 + 128 x 80
+// of the 384 x 168 the CTA starts with).
+// Every wait is bounded; one that gives up ends all roles and is counted.
+#include <cuda.h>
+
+#include <stdio.h>
+
+#include "attention.cuh"
+
+namespace iomb {
+namespace {
+
+constexpr uint32_t kThreads = 384;
+constexpr uint32_t kSoftmaxWarps = 8;
+constexpr uint32_t kTileRows = 128;
+constexpr uint32_t kMaxWidth = 128;
+constexpr uint32_t kMaxStages = 8;
+constexpr uint32_t kRingBytes = 128 * 1024;
+constexpr uint32_t kTmemColumns = 512;          // S of A and B: 0, 128; O of A and B: 256, 384
+constexpr uint32_t kMaskWords = kMaxTreeNodes / 32;
+constexpr float kRescale = 8.0f;                // in powers of two
+// Bounds of the waits: about a second, and a quarter of a minute where the other side may be
+// computing special rows again.
+constexpr long long kWaitCycles = 1ll << 31, kLongWaitCycles = 1ll << 35;
+
+__device__ unsigned int g_attention_timeouts;
+
+struct TcParams {
+    AttnParams a;
+    float scale_log2;           // scale * log2(e)
+    uint32_t stages;
+    // packed
+    uint32_t pack, tile_rows;   // heads per tile, rows per head of a tile
+    uint32_t head_tiles;        // tiles side by side: Hq / pack
+    // tree
+    uint32_t members;           // (head, node) pairs per key/value head
+    uint32_t alternate;         // both tiles hold the same rows
+    uint32_t pairs;             // tile pairs per key/value head
+    uint32_t row_cap;           // rows of one partial
+    uint64_t slot_floats;       // floats of one partial: row_cap * (D + 2), a multiple of eight
+    float* partial;             // [grid * 2][slot_floats]: O [row_cap][D], m, l
+};
+
+// ---- barriers, copies, tensor memory ---------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t shared_address(const void* p) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void bar_init(uint64_t* bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_address(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_address(bar)) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_address(bar)), "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ bool bar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(shared_address(bar)), "r"(parity) : "memory");
+    return done != 0;
+}
+// True when the phase completed; false when this wait or another of the CTA gave up.
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* stop,
+                                         long long limit = kWaitCycles) {
+    if (bar_test(bar, parity)) return true;
+    const long long start = clock64();
+    do {
+        if (bar_test(bar, parity)) return true;
+        if (*stop != 0) return false;
+    } while (clock64() - start < limit);
+    *stop = 1;
+    return false;
+}
+// 128 tokens x D of one plane: tile rows [tile_row, tile_row + 8), every tile column.
+__device__ __forceinline__ void copy_block(uint32_t dst, const CUtensorMap* map, uint64_t* bar, uint32_t tile_row,
+                                           uint32_t plane) {
+    asm volatile(
+            "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %3, %4, %3, %5}], [%2];"
+            ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(shared_address(bar)), "r"(0u), "r"(tile_row), "r"(plane)
+            : "memory");
+}
+
+__device__ __forceinline__ void tmem_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_load32(uint32_t address, uint32_t* r) {
+    asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+            "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+            "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+              "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+              "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+              "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+            : "r"(address));
+}
+__device__ __forceinline__ void tmem_store32(uint32_t address, const uint32_t* r) {
+    asm volatile(
+            "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+            "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+            "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+            ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+              "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+              "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+              "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
+              "r"(address)
+            : "memory");
+}
+__device__ __forceinline__ void tmem_load16(uint32_t address, uint32_t* r) {
+    asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+            "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+              "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+            : "r"(address));
+}
+__device__ __forceinline__ void tmem_store16(uint32_t address, const uint32_t* r) {
+    asm volatile(
+            "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+            "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+            ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+              "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+              "r"(address)
+            : "memory");
+}
+
+// Shared-memory operand with 32-byte swizzle. Groups of eight 32-byte rows lie 256 bytes apart
+// (stride offset); the leading offset is the distance of neighbouring 16-column pieces and only
+// the MN-major operand (V) uses it.
+__device__ __forceinline__ uint64_t operand_descriptor(uint32_t address, uint32_t leading_bytes) {
+    return static_cast<uint64_t>((address & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(leading_bytes >> 4) << 16)
+            | (static_cast<uint64_t>(256u >> 4) << 32) | (1ull << 46) | (6ull << 61);
+}
+// FP32 accumulators, A and B of one 16-bit format, M = 128, N = n; b_mn: B is MN-major.
+__device__ __forceinline__ uint32_t product_descriptor(uint32_t format, uint32_t n, bool b_mn) {
+    return (1u << 4) | (format << 7) | (format << 10) | ((b_mn ? 1u : 0u) << 16) | ((n >> 3) << 17)
+            | ((kTileRows >> 4) << 24);
+}
+__device__ __forceinline__ void mma_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t kind, bool accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(kind), "r"(accumulate ? 1u : 0u) : "memory");
+}
+__device__ __forceinline__ void mma_tensor(uint32_t d, uint32_t a, uint64_t b, uint32_t kind, bool accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(kind), "r"(accumulate ? 1u : 0u) : "memory");
+}
+// The barrier is reached when every matrix instruction issued so far has completed.
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
+                 ::"r"(shared_address(bar)) : "memory");
+}
+
+// Packed binary32 pairs: one instruction per two values.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// ---- the work of one CTA -----------------------------------------------------------------------------
+
+// A run of token blocks of one row set (a tile pair).
+struct Piece {
+    uint32_t b, kv_head, pair;  // sequence, key/value head, tile pair
+    uint32_t first_token;       // multiple of 16: the first block's first row of k and v
+    uint32_t blocks[2];         // per tile; equal in a tree call
+    uint32_t end;               // rows of the sequence end here (packed), live rows (tree)
+    uint32_t row0;              // packed: first row of tile A
+    uint32_t start;             // packed: first row of the sequence; tree: rows before the tree
+    uint32_t nodes;
+    uint32_t whole;             // tree: every block of the row set lies in this piece
+    uint32_t slot;              // tree: which of the CTA's partials
+};
+
+__device__ __forceinline__ uint32_t tree_blocks(const TreeExtent& e) {
+    return e.nodes == 0 ? 0 : (e.length + e.nodes + kKvBlock - 1) / kKvBlock;
+}
+
+// Walks the pieces of a CTA's range of token blocks: sequences, then (head, pair), then blocks.
+struct Walk {
+    uint32_t b, set, block;     // next piece begins here
+    uint64_t left;              // blocks of the range not walked yet
+};
+
+__device__ __forceinline__ bool next_piece(const TcParams& p, Walk& w, Piece& out) {
+    if (w.left == 0 || w.b >= p.a.batch) return false;
+    TreeExtent e = tree_extent(p.a, w.b);
+    uint32_t blocks = tree_blocks(e);
+    while (blocks == 0) {
+        if (++w.b >= p.a.batch) return false;
+        e = tree_extent(p.a, w.b);
+        blocks = tree_blocks(e);
+    }
+    const uint32_t rest = blocks - w.block;
+    const uint32_t take = w.left < rest ? static_cast<uint32_t>(w.left) : rest;
+    out.b = w.b;
+    out.kv_head = w.set / p.pairs;
+    out.pair = w.set % p.pairs;
+    out.first_token = w.block * kKvBlock;
+    out.blocks[0] = out.blocks[1] = take;
+    out.end = e.length + e.nodes;
+    out.row0 = 0;
+    out.start = e.length;
+    out.nodes = e.nodes;
+    out.whole = w.block == 0 && take == blocks ? 1u : 0u;
+    out.slot = w.block != 0 ? 0u : 1u;
+    w.left -= take;
+    w.block += take;
+    if (w.block == blocks) {
+        w.block = 0;
+        if (++w.set == p.a.hkv * p.pairs) {
+            w.set = 0;
+            ++w.b;
+        }
+    }
+    return true;
+}
+
+__device__ __forceinline__ uint64_t warp_sum64(uint64_t v) {
+    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    return v;
+}
+
+// Range [total * cta / ctas, total * (cta + 1) / ctas) of token blocks.
+__device__ __forceinline__ uint64_t range_begin(uint64_t total, uint32_t cta, uint32_t ctas) {
+    return total * cta / ctas;
+}
+
+// One warp: where this CTA's range begins.
+__device__ __forceinline__ Walk plan_walk(const TcParams& p, uint32_t cta, uint32_t ctas) {
+    const uint32_t lane = threadIdx.x & 31u;
+    const uint32_t sets = p.a.hkv * p.pairs;
+    uint64_t total = 0;
+    for (uint32_t b = lane; b < p.a.batch; b += 32) total += tree_blocks(tree_extent(p.a, b));
+    total = warp_sum64(total) * sets;
+    const uint64_t begin = range_begin(total, cta, ctas), end = range_begin(total, cta + 1, ctas);
+    Walk w{0, 0, 0, end - begin};
+    if (w.left == 0) return w;
+    uint64_t before = 0;
+    for (uint32_t base = 0; base < p.a.batch; base += 32) {
+        const uint32_t b = base + lane;
+        const uint32_t blocks = b < p.a.batch ? tree_blocks(tree_extent(p.a, b)) : 0;
+        uint64_t run = static_cast<uint64_t>(blocks) * sets;
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint64_t up = __shfl_up_sync(0xffffffffu, run, d);
+            if (lane >= static_cast<uint32_t>(d)) run += up;
+        }
+        const uint64_t mine_end = before + run, mine_begin = mine_end - static_cast<uint64_t>(blocks) * sets;
+        const uint32_t found = __ballot_sync(0xffffffffu, begin >= mine_begin && begin < mine_end);
+        if (found != 0) {
+            const int who = __ffs(found) - 1;
+            const uint64_t first = __shfl_sync(0xffffffffu, mine_begin, who);
+            const uint32_t n = __shfl_sync(0xffffffffu, blocks, who);
+            w.b = base + who;
+            w.set = static_cast<uint32_t>((begin - first) / n);
+            w.block = static_cast<uint32_t>((begin - first) % n);
+            return w;
+        }
+        before = __shfl_sync(0xffffffffu, mine_end, 31);
+    }
+    w.left = 0;     // not reached
+    return w;
+}
+
+// One warp: the tile pair of this CTA in a packed call. Units run over the sequences, each one's
+// row blocks from the last (the longest) to the first, heads innermost. False: nothing to do.
+__device__ __forceinline__ bool plan_packed(const TcParams& p, uint32_t unit, Piece& out, bool& ok) {
+    const uint32_t lane = threadIdx.x & 31u;
+    const uint32_t step = 2 * p.tile_rows;
+    const uint32_t head_tile = unit % p.head_tiles, wanted = unit / p.head_tiles;
+    constexpr uint32_t kChunks = 4;
+    uint32_t before = 0;
+    bool have = false;
+    ok = true;
+    for (uint32_t base = 0; base < p.a.batch; base += 32 * kChunks) {
+        uint32_t first[kChunks], last[kChunks];
+#pragma unroll
+        for (uint32_t c = 0; c < kChunks; ++c) {
+            const uint32_t s = base + c * 32 + lane;
+            first[c] = s < p.a.batch ? p.a.offsets[s] : 0;
+            last[c] = s < p.a.batch ? p.a.offsets[s + 1] : 0;
+        }
+#pragma unroll
+        for (uint32_t c = 0; c < kChunks; ++c) {
+            ok = ok && first[c] <= last[c] && last[c] <= p.a.rows;
+            const uint32_t rows = last[c] >= first[c] ? last[c] - first[c] : 0;
+            const uint32_t blocks = rows / step + (rows % step != 0 ? 1u : 0u);
+            uint32_t run = blocks;
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint32_t up = __shfl_up_sync(0xffffffffu, run, d);
+                if (lane >= static_cast<uint32_t>(d)) run += up;
+            }
+            const uint32_t mine_end = before + run, mine_begin = mine_end - blocks;
+            const uint32_t found = __ballot_sync(0xffffffffu, wanted >= mine_begin && wanted < mine_end);
+            if (found != 0 && !have) {
+                const int who = __ffs(found) - 1;
+                have = true;
+                out.start = __shfl_sync(0xffffffffu, first[c], who);
+                out.end = __shfl_sync(0xffffffffu, last[c], who);
+                out.row0 = out.start + __shfl_sync(0xffffffffu, mine_end - 1 - wanted, who) * step;
+            }
+            before = __shfl_sync(0xffffffffu, mine_end, 31);
+        }
+    }
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok || !have) return false;
+    out.b = 0;
+    out.kv_head = head_tile * p.pack / p.a.group;
+    out.pair = head_tile;
+    out.first_token = out.start / kTile * kTile;
+    for (uint32_t x = 0; x < 2; ++x) {
+        const uint32_t row = out.row0 + x * p.tile_rows;
+        const uint32_t last = min(out.end, row + p.tile_rows);      // one behind the tile's last row
+        out.blocks[x] = row < out.end ? (last - out.first_token + kKvBlock - 1) / kKvBlock : 0;
+    }
+    out.nodes = 0;
+    out.whole = 1;
+    out.slot = 0;
+    return true;
+}
+
+// Bits c of a word with low <= c <= high.
+__device__ __forceinline__ uint32_t range_word(int32_t low, int32_t high) {
+    const uint32_t up = high >= 31 ? 0xFFFFFFFFu : high < 0 ? 0u : (2u << high) - 1u;
+    const uint32_t down = low <= 0 ? 0xFFFFFFFFu : low > 31 ? 0u : 0xFFFFFFFFu << low;
+    return up & down;
+}
+
+// attend_row for one row of a tree or packed call, out of line: rare.
+template <class Leaf, bool TREE>
+__device__ __noinline__ void redo_row(const AttnParams& p, uint32_t b, uint32_t h, uint32_t row, uint32_t start) {
+    if constexpr (TREE) {
+        const int32_t* parents = p.parents != nullptr ? p.parents + static_cast<uint64_t>(b) * p.rows : nullptr;
+        attend_row<Leaf>(p, b, h, row, TreeRow{start, row, parents});
+    } else {
+        attend_row<Leaf>(p, b, h, row, CausalRows{start, row});
+    }
+}
+
+struct Shared {
+    uint64_t full[kMaxStages], empty[kMaxStages];
+    uint64_t scores[2], weights[2], done[2];    // S written, P written, O complete
+    uint64_t queries, drain;
+    uint32_t tmem, stop, run;
+    Piece piece;                                // packed
+    Walk walk;                                  // tree
+    float other[2][kTileRows];                  // m and l of tile B (alternate blocks)
+    uint32_t mask[kMaxTreeNodes * kMaskWords];  // ancestors and the node itself
+    int16_t parent[kMaxTreeNodes];
+};
+
+template <class Leaf, bool TREE>
+__global__ void __launch_bounds__(kThreads, 1)
+attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUtensorMap k_map,
+                    const __grid_constant__ CUtensorMap v_map) {
+    extern __shared__ __align__(1024) unsigned char dynamic[];
+    __shared__ Shared sh;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t width = p.a.width, slices = width / kTile;
+    const uint32_t block_bytes = width * kTileRows * 2;         // a Q tile, a K block, a V block
+    // The dynamic part starts behind the static one: round up to the swizzle's alignment.
+    const uint32_t q_base = (shared_address(dynamic) + 1023u) & ~1023u;
+    const uint32_t ring = q_base + (TREE && p.alternate ? 1u : 2u) * block_bytes;
+    volatile uint32_t* const stop = &sh.stop;
+
+    if (warp == 0) {
+        if constexpr (TREE) {
+            const Walk w = plan_walk(p, blockIdx.x, gridDim.x);
+            if (lane == 0) {
+                sh.walk = w;
+                sh.run = w.left != 0;
+            }
+        } else {
+            Piece piece;
+            bool ok;
+            const bool run = plan_packed(p, blockIdx.x, piece, ok);
+            if (lane == 0) {
+                sh.piece = piece;
+                sh.run = run;
+                if (blockIdx.x == 0) *p.a.status = ok ? 0u : 1u;
+            }
+        }
+    } else if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(shared_address(&sh.tmem)), "r"(kTmemColumns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    } else if (warp == 9 && lane == 0) {
+        for (uint32_t s = 0; s < kMaxStages; ++s) {
+            bar_init(&sh.full[s], 1);
+            bar_init(&sh.empty[s], 1);
+        }
+        for (uint32_t x = 0; x < 2; ++x) {
+            bar_init(&sh.scores[x], 1);
+            bar_init(&sh.weights[x], 4);
+            bar_init(&sh.done[x], 1);
+        }
+        bar_init(&sh.queries, kSoftmaxWarps);
+        bar_init(&sh.drain, 1);
+        sh.stop = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    tmem_before_sync();
+    __syncthreads();
+    tmem_after_sync();
+    if constexpr (TREE) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t tmem = sh.tmem;
+    const bool run = sh.run != 0;
+
+    if (warp < kSoftmaxWarps) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+
+    if (run && warp < kSoftmaxWarps) {
+        // ---- softmax, one thread per row ------------------------------------------------------------
+        const uint32_t x = warp / 4, m = threadIdx.x & 127u;
+        const uint32_t lanes = (warp & 3u) << 21;               // this warp's 32 tensor memory lanes
+        const uint32_t s_at = tmem + lanes + x * 128, o_at = tmem + lanes + 256 + x * 128;
+        const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
+        uint32_t steps_done = 0, pieces_done = 0;               // completed phases of this tile's barriers
+        Walk walk = sh.walk;
+        Piece piece = sh.piece;
+        bool go = TREE ? next_piece(p, walk, piece) : true;
+        while (go) {
+            const uint32_t n = TREE && p.alternate ? (piece.blocks[0] + 1 - x) / 2 : piece.blocks[x];
+            // This thread's row.
+            uint32_t head, row;
+            bool valid;
+            if constexpr (TREE) {
+                const uint32_t member = (p.alternate ? 0u : piece.pair * 256 + x * 128) + m;
+                head = piece.kv_head * p.a.group + member / p.a.rows;
+                row = member % p.a.rows;
+                valid = member < p.members && row < piece.nodes;
+            } else {
+                head = piece.pair * p.pack + m / p.tile_rows;
+                row = piece.row0 + x * p.tile_rows + m % p.tile_rows;
+                valid = row < piece.end;
+            }
+            const bool busy = __any_sync(0xffffffffu, valid) && n != 0;
+            if constexpr (TREE) {
+                // Ancestor masks, when the piece reaches the tree; nobody still reads the last piece's.
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (p.a.parents != nullptr && piece.first_token + piece.blocks[0] * kKvBlock > piece.start) {
+                    const int32_t* parents = p.a.parents + static_cast<uint64_t>(piece.b) * p.a.rows;
+                    for (uint32_t i = threadIdx.x; i < piece.nodes; i += 256) {
+                        sh.parent[i] = static_cast<int16_t>(max(-1, tree_parent(parents, static_cast<int32_t>(i))));
+                    }
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    for (uint32_t i = threadIdx.x; i < piece.nodes; i += 256) {
+                        uint32_t* words = sh.mask + i * kMaskWords;
+                        for (uint32_t w = 0; w < kMaskWords; ++w) words[w] = 0;
+                        for (int32_t at = static_cast<int32_t>(i); at >= 0; at = sh.parent[at]) {
+                            words[at / 32] |= 1u << (at % 32);
+                        }
+                    }
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                }
+            }
+            // Q: 32 bytes of a tile row per step, into the swizzled K-major operand.
+            if (!(TREE && p.alternate && x == 1) && n != 0) {
+                const uint64_t plane = attn_plane(p.a.q, piece.b, head);
+                const uint32_t dst = q_base + x * block_bytes + m * 32;
+                const uint32_t flip = ((m >> 2) & 1u) * 16;
+                for (uint32_t c = 0; c < slices; ++c) {
+                    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+                    if (valid) {
+                        const uint4* src = reinterpret_cast<const uint4*>(attn_piece(p.a.q, plane, row, c));
+                        lo = src[0];
+                        hi = src[1];
+                    }
+                    const uint32_t at = dst + c * 4096;
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at + flip), "r"(lo.x), "r"(lo.y), "r"(lo.z),
+                                 "r"(lo.w) : "memory");
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at + (16 - flip)), "r"(hi.x), "r"(hi.y),
+                                 "r"(hi.z), "r"(hi.w) : "memory");
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            }
+            __syncwarp();
+            if (lane == 0) bar_arrive(&sh.queries);
+
+            float top = __int_as_float(0xFF800000), sum = 0.0f;     // running maximum (of S) and sum
+            bool alive = true;
+            for (uint32_t step = 0; step < n; ++step) {
+                // (one answer per warp)
+                alive = __all_sync(0xffffffffu, bar_wait(&sh.scores[x], steps_done & 1u, stop));
+                if (!alive) break;
+                ++steps_done;
+                tmem_after_sync();
+                if (busy) {
+                    uint32_t s[128];
+                    tmem_load32(s_at, s);
+                    tmem_load32(s_at + 32, s + 32);
+                    tmem_load32(s_at + 64, s + 64);
+                    tmem_load32(s_at + 96, s + 96);
+                    const uint32_t block = TREE && p.alternate ? 2 * step + x : step;
+                    const uint32_t token = piece.first_token + block * kKvBlock;
+                    const bool masked = TREE ? token + kKvBlock > piece.start
+                                             : token < piece.start || token + kKvBlock > piece.row0 + x * p.tile_rows + 1;
+                    tmem_wait_load();
+                    if (masked) {
+                        uint32_t see[4];
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const int32_t first = static_cast<int32_t>(token) + 32 * w;
+                            if constexpr (!TREE) {
+                                see[w] = range_word(static_cast<int32_t>(piece.start) - first, static_cast<int32_t>(row) - first);
+                            } else if (p.a.parents == nullptr) {
+                                see[w] = range_word(0, static_cast<int32_t>(piece.start + row) - first);
+                            } else {
+                                see[w] = range_word(0, static_cast<int32_t>(piece.start) - 1 - first);
+                                const int32_t rel = first - static_cast<int32_t>(piece.start);
+                                if (valid && rel > -32 && rel < static_cast<int32_t>(kMaxTreeNodes)) {
+                                    const uint32_t* words = sh.mask + row * kMaskWords;
+                                    if (rel < 0) {
+                                        see[w] |= words[0] << -rel;
+                                    } else {
+                                        const uint32_t i = rel / 32;
+                                        see[w] |= __funnelshift_r(words[i], i + 1 < kMaskWords ? words[i + 1] : 0u, rel % 32);
+                                    }
+                                }
+                            }
+                            if (!valid) see[w] = 0;
+                        }
+#pragma unroll
+                        for (int c = 0; c < 128; ++c) {
+                            if (!((see[c / 32] >> (c % 32)) & 1u)) s[c] = 0xFF800000u;
+                        }
+                    }
+                    float best[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) best[i] = fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 4]));
+#pragma unroll
+                    for (int c = 8; c < 128; c += 8) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            best[i] = fmaxf(fmaxf(best[i], __uint_as_float(s[c + i])), __uint_as_float(s[c + i + 4]));
+                        }
+                    }
+                    const float high = fmaxf(top, fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])));
+                    // The first block, or a maximum that grew beyond what P may: a new reference.
+                    const bool fresh = top == __int_as_float(0xFF800000);
+                    const bool grow = !fresh && (high - top) * p.scale_log2 > kRescale;
+                    if (__any_sync(0xffffffffu, grow) && step != 0) {
+                        const float factor = grow ? exp2_fast((top - high) * p.scale_log2) : 1.0f;
+                        sum *= factor;
+                        for (uint32_t c = 0; c < slices; ++c) {
+                            uint32_t o[16];
+                            tmem_load16(o_at + c * 16, o);
+                            tmem_wait_load();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+                            tmem_store16(o_at + c * 16, o);
+                        }
+                    }
+                    if (fresh || grow) top = high;
+                    const float shift = top == __int_as_float(0xFF800000) ? 0.0f : -(top * p.scale_log2);
+                    const uint64_t shift2 = pair(shift, shift);
+                    uint64_t sums[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int c = 0; c < 128; c += 2) {
+                        float e0, e1;
+                        unpair(fma2(pair(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), scale2, shift2), e0, e1);
+                        e0 = exp2_fast(e0);
+                        e1 = exp2_fast(e1);
+                        sums[(c / 2) % 4] = add2(sums[(c / 2) % 4], pair(e0, e1));
+                        s[c / 2] = Leaf::pack(e0, e1);
+                    }
+                    tmem_store32(s_at, s);
+                    tmem_store32(s_at + 32, s + 32);
+                    float a, b;
+                    unpair(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])), a, b);
+                    sum += a + b;
+                    tmem_wait_store();
+                }
+                tmem_before_sync();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&sh.weights[x]);
+            }
+            if (alive && n != 0) {
+                alive = __all_sync(0xffffffffu, bar_wait(&sh.done[x], pieces_done & 1u, stop));
+                ++pieces_done;
+                tmem_after_sync();
+            }
+            // ---- results ---------------------------------------------------------------------------
+            const bool join = TREE && p.alternate;
+            const bool second = join && piece.blocks[0] > 1;       // tile B holds part of the sum
+            float mine = 1.0f, its = 0.0f;                          // factors of the two tiles' O
+            if (join) {
+                if (x == 1) {
+                    sh.other[0][m] = top;
+                    sh.other[1][m] = sum;
+                }
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (x == 0 && second) {
+                    const float top_b = sh.other[0][m], sum_b = sh.other[1][m];
+                    const float high = fmaxf(top, top_b);
+                    mine = sum == 0.0f ? 0.0f : exp2_fast((top - high) * p.scale_log2);
+                    its = sum_b == 0.0f ? 0.0f : exp2_fast((top_b - high) * p.scale_log2);
+                    sum = sum * mine + sum_b * its;
+                    top = high;
+                }
+            }
+            if (alive && busy && !(join && x == 1)) {
+                const uint32_t b_at = o_at + 128;
+                if (!TREE || piece.whole) {
+                    const float inverse = 1.0f / sum;
+                    bool bad = !(sum > 0.0f && sum <= 3.0e38f);
+                    const uint64_t plane = attn_plane(p.a.out, piece.b, 0);
+                    const uint32_t column = head * slices;
+                    for (uint32_t c = 0; c < slices; ++c) {
+                        uint32_t o[16], o2[16];
+                        tmem_load16(o_at + c * 16, o);
+                        if (second) tmem_load16(b_at + c * 16, o2);
+                        tmem_wait_load();
+                        uint32_t packed[8];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            float v = __uint_as_float(o[i]);
+                            if (second) {
+                                v = mine == 0.0f ? 0.0f : v * mine;
+                                if (its != 0.0f) v = __fmaf_rn(__uint_as_float(o2[i]), its, v);
+                            }
+                            v *= inverse;
+                            bad = bad || !(fabsf(v) <= 3.4028234e38f);
+                            o[i] = __float_as_uint(v);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            packed[i] = canonical_pair<Leaf>(Leaf::pack(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])));
+                        }
+                        if (valid) {
+                            store_u8_stream(attn_out_piece(p.a.out, plane, row, column + c),
+                                            make_uint4(packed[0], packed[1], packed[2], packed[3]),
+                                            make_uint4(packed[4], packed[5], packed[6], packed[7]));
+                        }
+                    }
+                    uint32_t again = __ballot_sync(0xffffffffu, bad && valid);
+                    while (again != 0) {
+                        const int who = __ffs(again) - 1;
+                        again &= again - 1;
+                        __syncwarp();
+                        redo_row<Leaf, TREE>(p.a, piece.b, __shfl_sync(0xffffffffu, head, who),
+                                             __shfl_sync(0xffffffffu, row, who), piece.start);
+                    }
+                } else if constexpr (TREE) {
+                    const uint32_t local = (p.alternate ? 0u : x * 128) + m;
+                    float* slot = p.partial + static_cast<uint64_t>(blockIdx.x * 2 + piece.slot) * p.slot_floats;
+                    for (uint32_t c = 0; c < slices; ++c) {
+                        uint32_t o[16], o2[16];
+                        tmem_load16(o_at + c * 16, o);
+                        if (second) tmem_load16(b_at + c * 16, o2);
+                        tmem_wait_load();
+                        if (second) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                float v = mine == 0.0f ? 0.0f : __uint_as_float(o[i]) * mine;
+                                if (its != 0.0f) v = __fmaf_rn(__uint_as_float(o2[i]), its, v);
+                                o[i] = __float_as_uint(v);
+                            }
+                        }
+                        if (valid) {
+                            uint4* to = reinterpret_cast<uint4*>(slot + static_cast<uint64_t>(local) * width + c * 16);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) to[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                        }
+                    }
+                    if (valid) {
+                        slot[static_cast<uint64_t>(p.row_cap) * width + local] = top;
+                        slot[static_cast<uint64_t>(p.row_cap) * (width + 1) + local] = sum;
+                    }
+                }
+            }
+            if constexpr (!TREE) break;
+            // Both tiles' results are out of tensor memory; one give-up ends both.
+            tmem_before_sync();
+            uint32_t over;
+            asm volatile("{\n\t.reg .pred mine, any;\n\tsetp.ne.u32 mine, %1, 0;\n\t"
+                         "barrier.cta.red.or.pred any, 1, 256, mine;\n\tselp.u32 %0, 1, 0, any;\n\t}"
+                         : "=r"(over) : "r"(alive && *stop == 0 ? 0u : 1u) : "memory");
+            if (over != 0) break;
+            go = next_piece(p, walk, piece);
+        }
+    } else if (run && warp == 8) {
+        // ---- matrix instructions, one thread -----------------------------------------------------------
+        if (lane == 0) {
+            const uint32_t kind_s = product_descriptor(Leaf::kFormat, kKvBlock, false);
+            const uint32_t kind_o = product_descriptor(Leaf::kFormat, width, true);
+            uint32_t taken = 0;             // ring slots consumed
+            uint32_t weights_seen[2] = {0, 0};
+            uint32_t pieces = 0;
+            bool alive = true;
+            Walk walk = sh.walk;
+            Piece piece = sh.piece;
+            bool go = TREE ? next_piece(p, walk, piece) : true;
+            auto wait_slot = [&](uint32_t& at) {
+                const uint32_t slot = taken % p.stages;
+                alive = alive && bar_wait(&sh.full[slot], (taken / p.stages) & 1u, stop);
+                ++taken;
+                at = slot;
+            };
+            auto score = [&](uint32_t x, uint32_t slot) {       // S of tile x = Q K^T
+                const uint32_t q = q_base + (TREE && p.alternate ? 0u : x) * block_bytes;
+                const uint32_t k = ring + slot * block_bytes;
+                for (uint32_t c = 0; c < slices; ++c) {
+                    mma_shared(tmem + x * 128, operand_descriptor(q + c * 4096, 0), operand_descriptor(k + c * 4096, 0),
+                               kind_s, c != 0);
+                }
+                mma_commit(&sh.scores[x]);
+            };
+            auto values = [&](uint32_t x, uint32_t slot, bool first) {      // O of tile x += P V
+                alive = alive && bar_wait(&sh.weights[x], weights_seen[x]++ & 1u, stop);
+                tmem_after_sync();
+                if (!alive) return;
+                const uint32_t v = ring + slot * block_bytes;
+                for (uint32_t t = 0; t < kKvBlock / kTile; ++t) {
+                    mma_tensor(tmem + 256 + x * 128, tmem + x * 128 + t * 8, operand_descriptor(v + t * 512, 4096), kind_o,
+                               !(first && t == 0));
+                }
+            };
+            while (go && alive) {
+                alive = bar_wait(&sh.queries, pieces++ & 1u, stop, kLongWaitCycles);
+                tmem_after_sync();
+                if (!alive) break;
+                if (TREE && p.alternate) {
+                    const uint32_t n = piece.blocks[0];
+                    uint32_t slot = 0;
+                    for (uint32_t i = 0; i < 2 && i < n && alive; ++i) {
+                        wait_slot(slot);
+                        if (!alive) break;
+                        score(i, slot);
+                        mma_commit(&sh.empty[slot]);
+                    }
+                    for (uint32_t i = 0; i < n && alive; ++i) {
+                        const uint32_t x = i & 1u;
+                        wait_slot(slot);
+                        if (!alive) break;
+                        values(x, slot, i < 2);
+                        if (!alive) break;
+                        mma_commit(&sh.empty[slot]);
+                        if (i + 2 >= n) {
+                            mma_commit(&sh.done[x]);
+                        } else {
+                            wait_slot(slot);
+                            if (!alive) break;
+                            score(x, slot);
+                            mma_commit(&sh.empty[slot]);
+                        }
+                    }
+                } else {
+                    const uint32_t n = max(piece.blocks[0], piece.blocks[1]);
+                    uint32_t k_slot = 0, v_slot = 0;
+                    wait_slot(k_slot);
+                    if (!alive) break;
+                    for (uint32_t x = 0; x < 2; ++x) {
+                        if (piece.blocks[x] != 0) score(x, k_slot);
+                    }
+                    mma_commit(&sh.empty[k_slot]);
+                    for (uint32_t i = 0; i < n && alive; ++i) {
+                        wait_slot(v_slot);
+                        if (i + 1 < n) wait_slot(k_slot);
+                        if (!alive) break;
+                        for (uint32_t x = 0; x < 2; ++x) {
+                            if (i >= piece.blocks[x]) continue;
+                            values(x, v_slot, i == 0);
+                            if (!alive) break;
+                            if (i + 1 < piece.blocks[x]) score(x, k_slot);
+                            else mma_commit(&sh.done[x]);
+                        }
+                        if (!alive) break;
+                        mma_commit(&sh.empty[v_slot]);
+                        if (i + 1 < n) mma_commit(&sh.empty[k_slot]);
+                    }
+                }
+                go = TREE ? next_piece(p, walk, piece) : false;
+            }
+            if (!alive) {
+                // Instructions still in flight end before the tensor memory is given back.
+                mma_commit(&sh.drain);
+                const long long start = clock64();
+                while (!bar_test(&sh.drain, 0) && clock64() - start < kWaitCycles) {}
+            }
+        }
+        __syncwarp();
+    } else if (run && warp == 9) {
+        // ---- copies, one thread -----------------------------------------------------------------------------
+        if (lane == 0) {
+            uint32_t issued = 0;
+            bool alive = true;
+            Walk walk = sh.walk;
+            Piece piece = sh.piece;
+            bool go = TREE ? next_piece(p, walk, piece) : true;
+            while (go && alive) {
+                const uint32_t k_plane = static_cast<uint32_t>(attn_plane(p.a.k, piece.b, piece.kv_head));
+                const uint32_t v_plane = static_cast<uint32_t>(attn_plane(p.a.v, piece.b, piece.kv_head));
+                const uint32_t first = piece.first_token / kTile;
+                auto fetch = [&](bool keys, uint32_t block) {
+                    const uint32_t slot = issued % p.stages;
+                    if (issued >= p.stages) alive = alive && bar_wait(&sh.empty[slot], (issued / p.stages - 1) & 1u, stop, kLongWaitCycles);
+                    if (!alive) return;
+                    bar_expect(&sh.full[slot], block_bytes);
+                    copy_block(ring + slot * block_bytes, keys ? &k_map : &v_map, &sh.full[slot],
+                               first + block * (kKvBlock / kTile), keys ? k_plane : v_plane);
+                    ++issued;
+                };
+                const uint32_t n = max(piece.blocks[0], piece.blocks[1]);
+                if (TREE && p.alternate) {
+                    // In the order the products take them: two key blocks ahead of the values.
+                    for (uint32_t i = 0; i < 2 && i < n && alive; ++i) fetch(true, i);
+                    for (uint32_t i = 0; i < n && alive; ++i) {
+                        fetch(false, i);
+                        if (i + 2 < n && alive) fetch(true, i + 2);
+                    }
+                } else {
+                    for (uint32_t i = 0; i < n && alive; ++i) {
+                        fetch(true, i);
+                        if (alive) fetch(false, i);
+                    }
+                }
+                go = TREE ? next_piece(p, walk, piece) : false;
+            }
+            // No copy and no barrier arrival outlives the CTA.
+            const uint32_t tail = issued < p.stages ? issued : p.stages;
+            for (uint32_t i = issued - tail; i < issued; ++i) {
+                uint64_t* bar = alive ? &sh.empty[i % p.stages] : &sh.full[i % p.stages];
+                const long long start = clock64();
+                while (!bar_test(bar, (i / p.stages) & 1u) && clock64() - start < kWaitCycles) {
+                    if (alive && *stop != 0) alive = false;
+                    bar = alive ? bar : &sh.full[i % p.stages];
+                }
+            }
+        }
+        __syncwarp();
+    }
+    if constexpr (TREE) {
+        // (behind the copies, beside the last products)
+        if (warp == 9 && blockIdx.x == 0) warp_report_tree(p.a);
+    }
+    tmem_before_sync();
+    __syncthreads();
+    tmem_after_sync();
+    if (warp == 8) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns));
+        if (lane == 0 && sh.stop != 0) atomicAdd(&g_attention_timeouts, 1u);
+    }
+}
+
+// Joins the partial sums of row sets whose blocks lie in several ranges: a warp per row, the
+// ranges in order. Reads a few KB per row; bound by the latency of two dependent reads.
+constexpr uint32_t kJoinRows = 32, kJoinWarps = 4;
+
+template <class Leaf>
+__global__ void __launch_bounds__(kJoinWarps * 32)
+attention_join_kernel(const __grid_constant__ TcParams p, uint32_t ctas) {
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const uint32_t sets = p.a.hkv * p.pairs;
+    const uint32_t b = blockIdx.x / sets, set = blockIdx.x % sets;
+    __shared__ uint64_t shared_total[kJoinWarps], shared_before[kJoinWarps];
+    uint64_t total = 0, before = 0;
+    for (uint32_t i = threadIdx.x; i < p.a.batch; i += kJoinWarps * 32) {
+        const uint32_t n = tree_blocks(tree_extent(p.a, i));
+        total += n;
+        if (i < b) before += n;
+    }
+    total = warp_sum64(total);
+    before = warp_sum64(before);
+    if (lane == 0) {
+        shared_total[warp] = total;
+        shared_before[warp] = before;
+    }
+    __syncthreads();
+    total = before = 0;
+    for (uint32_t w = 0; w < kJoinWarps; ++w) {
+        total += shared_total[w];
+        before += shared_before[w];
+    }
+    const TreeExtent e = tree_extent(p.a, b);
+    const uint32_t blocks = tree_blocks(e);
+    // (every CTA waits, also one with nothing to do: the join ends after the ranges)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (blocks == 0) return;
+    total *= sets;
+    const uint64_t first = before * sets + static_cast<uint64_t>(set) * blocks, end = first + blocks;
+    // The ranges that hold block `first` and block `end - 1`.
+    auto owner = [&](uint64_t block) {
+        uint32_t c = static_cast<uint32_t>(block * ctas / total);
+        while (c + 1 < ctas && range_begin(total, c + 1, ctas) <= block) ++c;
+        while (c > 0 && range_begin(total, c, ctas) > block) --c;
+        return c;
+    };
+    const uint32_t c0 = owner(first), c1 = owner(end - 1);
+    if (c0 == c1) return;                       // one range wrote the result itself
+    const uint32_t width = p.a.width;
+    const uint32_t kv_head = set / p.pairs, offset = (set % p.pairs) * 256;
+    const uint32_t rows = min(p.row_cap, p.members - offset);
+    for (uint32_t r = blockIdx.y * kJoinRows + warp; r < min(rows, (blockIdx.y + 1) * kJoinRows); r += kJoinWarps) {
+        const uint32_t member = offset + r, node = member % p.a.rows;
+        const uint32_t head = kv_head * p.a.group + member / p.a.rows;
+        if (node >= e.nodes) continue;
+        // (the row set began in range c0: its second partial unless it began exactly there)
+        auto slot = [&](uint32_t c) {
+            const uint32_t which = range_begin(total, c, ctas) > first ? 0u : 1u;
+            return p.partial + (static_cast<uint64_t>(c) * 2 + which) * p.slot_floats;
+        };
+        float top = __int_as_float(0xFF800000);
+        for (uint32_t c = c0 + lane; c <= c1; c += 32) {
+            const float* at = slot(c);
+            if (at[static_cast<uint64_t>(p.row_cap) * (width + 1) + r] != 0.0f) {
+                top = fmaxf(top, at[static_cast<uint64_t>(p.row_cap) * width + r]);
+            }
+        }
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        float sum = 0.0f, o[kMaxWidth / 32] = {};
+        for (uint32_t base = c0; base <= c1; base += 32) {
+            // Every lane has one range's factor ready; all lanes then add it up in order.
+            float factor = 0.0f, part = 0.0f;
+            if (base + lane <= c1) {
+                const float* at = slot(base + lane);
+                part = at[static_cast<uint64_t>(p.row_cap) * (width + 1) + r];
+                if (part != 0.0f) {
+                    factor = exp2_fast((at[static_cast<uint64_t>(p.row_cap) * width + r] - top) * p.scale_log2);
+                }
+            }
+            const uint32_t count = min(32u, c1 - base + 1);
+            for (uint32_t i = 0; i < count; ++i) {
+                const float f = __shfl_sync(0xffffffffu, factor, i), l = __shfl_sync(0xffffffffu, part, i);
+                if (l == 0.0f) continue;        // nothing seen in that range
+                sum = __fmaf_rn(l, f, sum);
+                const float* at = slot(base + i) + static_cast<uint64_t>(r) * width;
+#pragma unroll
+                for (uint32_t k = 0; k < kMaxWidth / 32; ++k) {
+                    if (lane + 32 * k < width) o[k] = __fmaf_rn(at[lane + 32 * k], f, o[k]);
+                }
+            }
+        }
+        const float inverse = 1.0f / sum;
+        bool bad = !(sum > 0.0f && sum <= 3.0e38f);
+#pragma unroll
+        for (uint32_t k = 0; k < kMaxWidth / 32; ++k) {
+            o[k] *= inverse;
+            bad = bad || !(fabsf(o[k]) <= 3.4028234e38f);
+        }
+        if (__any_sync(0xffffffffu, bad)) {
+            redo_row<Leaf, true>(p.a, b, head, node, e.length);
+            continue;
+        }
+        const uint64_t plane = attn_plane(p.a.out, b, 0);
+#pragma unroll
+        for (uint32_t k = 0; k < kMaxWidth / 32; ++k) {
+            const uint32_t d = lane + 32 * k;
+            if (d >= width) break;
+            const uint32_t column = head * width + d;
+            *(reinterpret_cast<uint16_t*>(attn_out_piece(p.a.out, plane, node, column / kTile)) + column % kTile) =
+                    static_cast<uint16_t>(canonical_pair<Leaf>(Leaf::pack(o[k], 0.0f)));
+        }
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+    static const EncodeTiled entry = [] {
+        void* symbol = nullptr;
+        cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &symbol, cudaEnableDefault, &found) != cudaSuccess
+                || found != cudaDriverEntryPointSuccess) {
+            (void)cudaGetLastError();
+            return static_cast<EncodeTiled>(nullptr);
+        }
+        return reinterpret_cast<EncodeTiled>(symbol);
+    }();
+    return entry;
+}
+
+// The owner's storage as (column in tile, row in tile, tile row, tile column, plane): a box of
+// eight tile rows and every tile column lands as [tile column][tile row][16][32 bytes].
+bool make_block_map(CUtensorMap* map, const AttnOperand& o) {
+    const EncodeTiled encode = encode_tiled();
+    if (encode == nullptr) return false;
+    const uint64_t tile_bytes = kTileSlots * 2, band_bytes = o.tile_cols * tile_bytes;
+    const cuuint64_t dims[5] = {kTile, kTile, o.tile_rows, o.tile_cols, o.planes};
+    const cuuint64_t strides[4] = {kTile * 2, band_bytes, tile_bytes, o.tile_rows * band_bytes};
+    const cuuint32_t box[5] = {kTile, kTile, kKvBlock / kTile, o.tile_cols, 1};
+    const cuuint32_t element_strides[5] = {1, 1, 1, 1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, o.base, dims, strides, box, element_strides,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_32B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The tree call's shape: which rows share a tile, how many ranges.
+struct TreeShape {
+    uint32_t members, alternate, pairs, row_cap, ctas;
+    bool cut;               // a row set's blocks may lie in several ranges
+    uint64_t slot_floats;
+};
+TreeShape tree_shape(const AttnParams& a) {
+    TreeShape t{};
+    t.members = a.group * a.rows;
+    t.alternate = t.members <= kTileRows ? 1u : 0u;
+    t.pairs = t.alternate ? 1 : (t.members + 2 * kTileRows - 1) / (2 * kTileRows);
+    t.row_cap = t.members < 2 * kTileRows ? t.members : 2 * kTileRows;
+    const uint64_t blocks = (static_cast<uint64_t>(a.cache_rows) + kKvBlock - 1) / kKvBlock;
+    const uint64_t all = static_cast<uint64_t>(a.batch) * a.hkv * t.pairs * blocks;
+    t.ctas = grid_for(all, 1);
+    t.cut = blocks > 1;
+    t.slot_floats = (static_cast<uint64_t>(t.row_cap) * (a.width + 2) + 7) / 8 * 8;
+    return t;
+}
+
+uint32_t shared_bytes(const AttnParams& a, bool alternate, uint32_t* stages) {
+    const uint32_t block = a.width * kTileRows * 2;
+    *stages = kRingBytes / block < kMaxStages ? kRingBytes / block : kMaxStages;
+    return 1024 + ((alternate ? 1u : 2u) + *stages) * block;
+}
+
+}  // namespace
+
+bool attention_tc_takes(const AttnParams& p) {
+    return p.width % kTile == 0 && p.width <= kMaxWidth && p.k.planes <= 0x7FFFFFFFull && p.v.planes <= 0x7FFFFFFFull;
+}
+
+uint64_t attention_tc_workspace(const AttnParams& a) {
+    const TreeShape t = tree_shape(a);
+    if (!t.cut) return 0;
+    return static_cast<uint64_t>(t.ctas) * 2 * t.slot_floats * sizeof(float);
+}
+
+template <class Leaf, bool TREE>
+static int launch_leaf(TcParams& p, uint32_t grid, uint32_t dynamic, const TreeShape* shape, cudaStream_t stream) {
+    CUtensorMap k_map, v_map;
+    if (!make_block_map(&k_map, p.a.k) || !make_block_map(&v_map, p.a.v)) {
+        return fail(IOMB_ERR_DEVICE, "attention: the tensor map could not be encoded");
+    }
+    const int rc = allow_full_shared_memory(reinterpret_cast<const void*>(&attention_tc_kernel<Leaf, TREE>));
+    if (rc != IOMB_OK) return rc;
+    attention_tc_kernel<Leaf, TREE><<<grid, kThreads, dynamic, stream>>>(p, k_map, v_map);
+    if constexpr (TREE) {
+        if (shape->cut) {
+            const int status = check_launch("sdpa_tree launch");
+            if (status != IOMB_OK) return status;
+            // The join's CTAs may be set up while the last ranges finish; they wait before they read.
+            cudaLaunchConfig_t config{};
+            config.gridDim = dim3(p.a.batch * p.a.hkv * p.pairs, (p.row_cap + kJoinRows - 1) / kJoinRows);
+            config.blockDim = dim3(kJoinWarps * 32);
+            config.stream = stream;
+            cudaLaunchAttribute early{};
+            early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            early.val.programmaticStreamSerializationAllowed = 1;
+            config.attrs = &early;
+            config.numAttrs = 1;
+            if (cudaLaunchKernelEx(&config, attention_join_kernel<Leaf>, static_cast<const TcParams&>(p), grid) != cudaSuccess) {
+                return check_launch("sdpa_tree join launch");
+            }
+        }
+    }
+    return check_launch(TREE ? "sdpa_tree launch" : "sdpa_packed launch");
+}
+
+int launch_attention_tc(const AttnParams& a, bool tree, bool bf16, void* workspace, cudaStream_t stream) {
+    TcParams p{};
+    p.a = a;
+    p.scale_log2 = a.scale * 1.4426950408889634f;
+    if (tree) {
+        const TreeShape t = tree_shape(a);
+        p.members = t.members;
+        p.alternate = t.alternate;
+        p.pairs = t.pairs;
+        p.row_cap = t.row_cap;
+        p.slot_floats = t.slot_floats;
+        p.partial = static_cast<float*>(workspace);
+        const uint32_t dynamic = shared_bytes(a, t.alternate != 0, &p.stages);
+        return bf16 ? launch_leaf<LeafBf16, true>(p, t.ctas, dynamic, &t, stream)
+                    : launch_leaf<LeafF16, true>(p, t.ctas, dynamic, &t, stream);
+    }
+    // As many heads of a group per tile as divide it, up to eight (16 rows each): heads of one
+    // group read the same tokens, and short sequences fill the tile.
+    p.pack = 1;
+    while (p.pack < 8 && a.group % (p.pack * 2) == 0) p.pack *= 2;
+    p.tile_rows = kTileRows / p.pack;
+    p.head_tiles = a.hq / p.pack;
+    p.members = 0;
+    p.pairs = 1;
+    const uint64_t units = (static_cast<uint64_t>(a.rows) / (2 * p.tile_rows) + (a.batch < a.rows ? a.batch : a.rows))
+            * p.head_tiles;
+    if (units > 0x7FFFFFFFull) return fail(IOMB_ERR_UNSUPPORTED, "sdpa_packed: too many rows for one launch");
+    const uint32_t dynamic = shared_bytes(a, false, &p.stages);
+    return bf16 ? launch_leaf<LeafBf16, false>(p, static_cast<uint32_t>(units), dynamic, nullptr, stream)
+                : launch_leaf<LeafF16, false>(p, static_cast<uint32_t>(units), dynamic, nullptr, stream);
+}
+
+int prepare_attention_kernels() {
+    for (const void* kernel : {reinterpret_cast<const void*>(&attention_tc_kernel<LeafBf16, true>),
+                               reinterpret_cast<const void*>(&attention_tc_kernel<LeafF16, true>),
+                               reinterpret_cast<const void*>(&attention_tc_kernel<LeafBf16, false>),
+                               reinterpret_cast<const void*>(&attention_tc_kernel<LeafF16, false>)}) {
+        const int rc = allow_full_shared_memory(kernel);
+        if (rc != IOMB_OK) return rc;
+    }
+    return IOMB_OK;
+}
+
+}  // namespace iomb
+
+extern "C" int iomb_sdpa_wait_timeouts(unsigned int* count) {
+    using namespace iomb;
+    if (count == nullptr) return fail(IOMB_ERR_INVALID_ARGUMENT, "null result");
+    if (cudaMemcpyFromSymbol(count, g_attention_timeouts, sizeof *count) != cudaSuccess) {
+        return check_launch("attention timeout counter");
+    }
+    return IOMB_OK;
+}

@@ -294,6 +294,7 @@ int iomb_prepare_device(void* stream) {
     int status = iomb::prepare_rmsnorm_kernels();
     if (status == IOMB_OK) status = iomb::prepare_rmsnorm_long_kernels();
     if (status == IOMB_OK) status = iomb::prepare_sdpa_kernels();
+    if (status == IOMB_OK) status = iomb::prepare_attention_kernels();
     if (status == IOMB_OK) status = iomb::prepare_silu(static_cast<cudaStream_t>(stream));
     return status;
 }

@@ -60,6 +60,7 @@ int prepare_rmsnorm_kernels();
 int prepare_rmsnorm_long_kernels();
 int prepare_silu(cudaStream_t stream);
 int prepare_sdpa_kernels();
+int prepare_attention_kernels();
 
 // Grid size for grid-stride kernels: enough CTAs to fill every SM
 // `ctas_per_sm` times, never more than `work_items`.
