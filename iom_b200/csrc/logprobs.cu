@@ -40,7 +40,8 @@ struct ScoreParams {
     Operand logits, tokens, logprob, entropy, top_value, top_token;
     Leading leading;
     uint32_t rows, vocab, top;
-    uint32_t bands;                         // per plane
+    uint32_t bands;                         // row groups per plane
+    uint32_t group_log;                     // log2 of the rows of a group (at most a tile's 16)
     uint32_t has_entropy;
     uint32_t token_bits, token_signed;
     uint32_t* status;
@@ -74,7 +75,8 @@ struct ScoreF32 {
     }
 };
 
-// Eight columns of one row of a tile: 16 or 32 bytes.
+// Eight columns of one row of a tile: 16 or 32 bytes. (Volatile and without a condition, so that a
+// group of loads stays in front of the first use: sunk into their uses they would wait one by one.)
 template <class Leaf>
 struct Chunk {
     uint4 lo, hi;
@@ -84,7 +86,8 @@ struct Chunk {
                          : "=r"(lo.x), "=r"(lo.y), "=r"(lo.z), "=r"(lo.w), "=r"(hi.x), "=r"(hi.y), "=r"(hi.z), "=r"(hi.w)
                          : "l"(at));
         } else {
-            lo = load_u4(at);
+            asm volatile("ld.global.v4.b32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(lo.x), "=r"(lo.y), "=r"(lo.z), "=r"(lo.w) : "l"(at));
         }
     }
     __device__ __forceinline__ void values(float (&x)[8]) const {
@@ -180,12 +183,23 @@ __device__ __forceinline__ RunningSum shuffle_sum(const RunningSum& s, int dista
                       __shfl_xor_sync(0xffffffffu, s.t, distance)};
 }
 
+// log2 of the rows of a tile a warp's lanes are spread over: as many as there are, so that they
+// load 16 / rows tiles side by side; for short rows more (lanes without a row idle), so that
+// there are at least 16 spans and with them more groups of columns than best tokens.
+__host__ __device__ __forceinline__ uint32_t lane_spread(uint32_t live, uint32_t tile_cols) {
+    uint32_t log = live > 8 ? 4 : live > 4 ? 3 : live > 2 ? 2 : live > 1 ? 1 : 0;
+    while (log < 4 && (tile_cols >> (4 - log)) < 16) ++log;
+    return log;
+}
+
 // The owner's side: rows rank, rank + cluster, ... of the band, row i / cluster in these arrays.
 struct ScoreShared {
     RunningSum sums[kTile * kScoreWarps];       // [rows here][warps of the cluster]
     float groups[kTile * 64];                   // [rows here][groups]: 16 x 64, 8 x 128, 4 x 64, 2 x 128
-    float tau[kTile], top[kTile], log_z[kTile];
+    float top[kTile], log_z[kTile];
     uint32_t odd[kTile], count[kTile];
+    float tau[kTile];                           // of every row of the group, from the rows' owners
+    uint8_t hot[kScoreWarps][32 * kSlots];      // a warp's (slot, lane) pairs that reach tau
     unsigned long long candidates[kTile][kCandidates];
 };
 
@@ -240,21 +254,22 @@ score_kernel(const __grid_constant__ ScoreParams p) {
     // Nobody writes into a neighbour before all have started and zeroed their counts.
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     const uint64_t index = unit / p.bands;
-    const uint32_t band = unit % p.bands;
-    const uint32_t live = min(kTile, p.rows - band * kTile);
+    const uint32_t first_row = (unit % p.bands) << p.group_log;
+    const uint32_t live = min(1u << p.group_log, p.rows - first_row);
     const uint64_t plane = operand_plane(p.logits, p.leading, index);
     // Lanes: half a tile row each; `spread` rows of a tile, 16 / spread tiles side by side.
-    const uint32_t spread_log = live > 8 ? 4 : live > 4 ? 3 : live > 2 ? 2 : live > 1 ? 1 : 0;
+    const uint32_t spread_log = lane_spread(live, p.logits.tile_cols);
     const uint32_t row = (lane >> 1) & ((1u << spread_log) - 1u);
     const uint32_t side = lane >> (1 + spread_log), sides_log = 4 - spread_log;
     const uint32_t half = lane & 1u;
     const uint32_t warps = ctas * kScoreWarps, my_warp = rank * kScoreWarps + warp;
     const uint32_t tile_cols = p.logits.tile_cols;
-    const unsigned char* const base = p.logits.base
-            + (plane * p.logits.tile_rows + band) * tile_cols * static_cast<uint64_t>(kTileSlots * Leaf::kBytes)
-            + row * (kTile * Leaf::kBytes) + half * (8 * Leaf::kBytes);
+    const unsigned char* const row_base = p.logits.base
+            + (plane * p.logits.tile_rows + first_row / kTile) * tile_cols * static_cast<uint64_t>(kTileSlots * Leaf::kBytes)
+            + first_row % kTile * (kTile * Leaf::kBytes);
+    const unsigned char* const base = row_base + min(row, live - 1) * (kTile * Leaf::kBytes) + half * (8 * Leaf::kBytes);
     const uint32_t spans = (tile_cols + (1u << sides_log) - 1) >> sides_log;    // a warp's loads side by side
-    const bool mine = row < live;
+    const bool mine = row < live;              // (lanes of rows that are not there read the last one)
 
     float m = kNone, less = 0.0f;               // running maximum, and what is subtracted (0 while -inf)
     uint64_t z2 = 0, t2 = 0;                    // sums over even and odd columns
@@ -267,12 +282,12 @@ score_kernel(const __grid_constant__ ScoreParams p) {
 #pragma unroll
         for (uint32_t u = 0; u < kSlots; ++u) {
             const uint32_t tile = ((first + u * warps) << sides_log) + side;
-            if (mine && tile < tile_cols) chunk[u].load(base + static_cast<uint64_t>(tile) * (kTileSlots * Leaf::kBytes));
+            chunk[u].load(base + static_cast<uint64_t>(min(tile, tile_cols - 1)) * (kTileSlots * Leaf::kBytes));
         }
 #pragma unroll
         for (uint32_t u = 0; u < kSlots; ++u) {
             const uint32_t tile = ((first + u * warps) << sides_log) + side;
-            if (!mine || tile >= tile_cols) continue;
+            if (tile >= tile_cols) continue;
             float x[8];
             chunk[u].values(x);
             const uint32_t column = tile * kTile + half * 8;
@@ -363,34 +378,34 @@ score_kernel(const __grid_constant__ ScoreParams p) {
     cluster.sync();
     // ---- the owners' rows ---------------------------------------------------------------------------
     for (uint32_t at = warp; rank + at * ctas < live; at += kScoreWarps) {
-        const uint32_t r = rank + at * ctas, logical = band * kTile + r;
+        const uint32_t r = rank + at * ctas, logical = first_row + r;
         RunningSum all{kNone, 0.0f, 0.0f};
         for (uint32_t w = lane; w < warps; w += 32) all = join_sums(all, sh.sums[at * warps + w]);
         for (int d = 16; d > 0; d >>= 1) all = join_sums(all, shuffle_sum(all, d));
         const bool odd = all.m == kNone || all.z != all.z || all.m == kInf;
         const float log_z = logf(all.z);
         if (p.top != 0) {
-            // tau: the K-th largest group maximum, groups in order among equals.
+            // tau: the K-th largest group maximum, or a little less: the largest value of 16 leading
+            // bits (in the order of the keys) that at least K of them reach.
             const float* g = sh.groups + at * groups;
-            float value[kMaxGroups / 32];
-            uint32_t above[kMaxGroups / 32] = {};
-#pragma unroll
-            for (uint32_t i = 0; i < kMaxGroups / 32; ++i) value[i] = i * 32 < groups ? g[i * 32 + lane] : kNone;
-            for (uint32_t j = 0; j < groups; ++j) {
-                const float other = g[j];
-#pragma unroll
-                for (uint32_t i = 0; i < kMaxGroups / 32; ++i) {
-                    above[i] += other > value[i] || (other == value[i] && j < i * 32 + lane) ? 1u : 0u;
-                }
-            }
-            if (lane == 0) sh.tau[at] = kNone;
-            __syncwarp();
+            uint32_t order[kMaxGroups / 32];
 #pragma unroll
             for (uint32_t i = 0; i < kMaxGroups / 32; ++i) {
-                if (i * 32 < groups && above[i] == p.top - 1) sh.tau[at] = value[i];
+                order[i] = i * 32 < groups ? static_cast<uint32_t>(score_key(g[i * 32 + lane], 0) >> 32) : 0;
             }
+            uint32_t reached = 0;
+            for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
+                uint32_t n = 0;
+#pragma unroll
+                for (uint32_t i = 0; i < kMaxGroups / 32; ++i) n += __popc(__ballot_sync(0xffffffffu, order[i] >= (reached | bit)));
+                if (n >= p.top) reached |= bit;
+            }
+            // (the smallest orders are NaN's as a float: nothing is ruled out by it)
+            float tau = key_value(static_cast<uint64_t>(reached) << 32);
+            if (tau != tau) tau = kNone;
+            if (odd) tau = kInf;                        // (no candidates: the row is walked)
+            if (lane < ctas) cluster.map_shared_rank(&sh, lane)->tau[r] = tau;
             if (lane == 0) {
-                if (odd) sh.tau[at] = kInf;             // (no candidates: the row is walked)
                 sh.top[at] = all.m;
                 sh.log_z[at] = log_z;
                 sh.odd[at] = odd;
@@ -413,33 +428,58 @@ score_kernel(const __grid_constant__ ScoreParams p) {
     if (p.top == 0) return;                             // (nobody reads a neighbour any more)
     cluster.sync();
     // ---- candidates: the slots that reach tau, once more ---------------------------------------------
-    if (mine) {
-        ScoreShared* const there = cluster.map_shared_rank(&sh, owner);
-        const float tau = there->tau[place];
+    {
+        const float tau = sh.tau[row];
+        uint32_t hot = 0;
 #pragma unroll
         for (uint32_t u = 0; u < kSlots; ++u) {
-            if (!(best[u] >= tau) || best[u] == kNone) continue;
-            for (uint32_t span = my_warp + u * warps; span < spans; span += kSlots * warps) {
-                const uint32_t tile = (span << sides_log) + side;
-                if (tile >= tile_cols) break;
+            const bool reaches = mine && best[u] >= tau && best[u] != kNone;
+            const uint32_t who = __ballot_sync(0xffffffffu, reaches);
+            if (reaches) sh.hot[warp][hot + __popc(who & ((1u << lane) - 1u))] = static_cast<uint8_t>(u * 32 + lane);
+            hot += __popc(who);
+        }
+        __syncwarp();
+        // Eight lanes per pair: each takes every eighth of the pair's chunks, so that a pair costs
+        // one wait for memory and not one per chunk.
+        for (uint32_t first = 0; first < hot; first += 4) {
+            const uint32_t at = first + lane / 8;
+            const uint32_t pair = sh.hot[warp][min(at, hot - 1)];
+            const uint32_t its_lane = pair % 32, u = pair / 32;
+            const uint32_t its_row = (its_lane >> 1) & ((1u << spread_log) - 1u), its_side = its_lane >> (1 + spread_log);
+            const float its_tau = sh.tau[its_row];
+            ScoreShared* const there = cluster.map_shared_rank(&sh, its_row % ctas);
+            const uint32_t its_place = its_row / ctas;
+            const unsigned char* const from = row_base + its_row * (kTile * Leaf::kBytes) + (its_lane & 1u) * (8 * Leaf::kBytes);
+            const uint32_t step = kSlots * warps;
+            for (uint32_t span = my_warp + u * warps + (lane % 8) * step; ; span += 8 * step) {
+                const uint32_t tile = (span << sides_log) + its_side;
+                const bool there_is = at < hot && span < spans && tile < tile_cols;
+                if (!__any_sync(0xffffffffu, there_is)) break;
+                if (!there_is) continue;
                 Chunk<Leaf> chunk;
-                chunk.load(base + static_cast<uint64_t>(tile) * (kTileSlots * Leaf::kBytes));
+                chunk.load(from + static_cast<uint64_t>(tile) * (kTileSlots * Leaf::kBytes));
                 float x[8];
                 chunk.values(x);
-                const uint32_t column = tile * kTile + half * 8;
+                const uint32_t column = tile * kTile + (its_lane & 1u) * 8;
+                uint32_t reach = 0;
 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i) {
-                    if (x[i] >= tau && x[i] > kNone && column + i < p.vocab) {
-                        const uint32_t n = atomicAdd(&there->count[place], 1u);
-                        if (n < kCandidates) there->candidates[place][n] = score_key(x[i], column + i);
-                    }
+                    reach |= (x[i] >= its_tau && x[i] > kNone && column + i < p.vocab ? 1u : 0u) << i;
+                }
+                if (reach == 0) continue;
+                uint32_t n = atomicAdd(&there->count[its_place], static_cast<uint32_t>(__popc(reach)));
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) {
+                    if (!((reach >> i) & 1u)) continue;
+                    if (n < kCandidates) there->candidates[its_place][n] = score_key(x[i], column + i);
+                    ++n;
                 }
             }
         }
     }
     cluster.sync();
     for (uint32_t at = warp; rank + at * ctas < live; at += kScoreWarps) {
-        const uint32_t r = rank + at * ctas, logical = band * kTile + r;
+        const uint32_t r = rank + at * ctas, logical = first_row + r;
         const bool odd = sh.odd[at] != 0;
         const uint32_t n = sh.count[at];
         const uint64_t value_plane = operand_plane(p.top_value, p.leading, index);
@@ -553,14 +593,20 @@ extern "C" int iomb_token_logprobs(const iomb_view* logits, const iomb_view* tok
     p.token_bits = facts[1].bits;
     p.token_signed = tokens->dtype == IOMB_I32 || tokens->dtype == IOMB_I64;
     p.status = status;
-    p.bands = static_cast<uint32_t>(facts[0].tile_rows);
-    // CTAs per band: enough that each warp still has a few loads (four in flight), for few bands
-    // as for many (a long row is read at the rate of several SMs, and the more groups of columns,
-    // the less of it is read twice).
-    const uint32_t rows_spread = rows > 8 ? 16 : rows > 4 ? 8 : rows > 2 ? 4 : rows > 1 ? 2 : 1;
-    const uint64_t spans = facts[0].tile_cols * rows_spread / 16;
-    uint32_t ctas = 1;
-    while (ctas < kMaxCluster && spans >= static_cast<uint64_t>(ctas) * 2 * kScoreWarps * kSlots) ctas *= 2;
+    // Rows per cluster: a tile's 16 (whole tiles in one read), fewer while the clusters would leave
+    // SMs idle: 64 rows of 32000 BF16 take 18 us in groups of 16 and 9.7 in groups of two. CTAs
+    // per cluster: up to eight while each warp still has two loads to do (a row is then read at the
+    // rate of several SMs, and the more groups of columns, the less of it is read twice).
+    uint32_t group_log = 4, ctas = 1;
+    for (;; --group_log) {
+        const uint32_t most = rows < (1ull << group_log) ? static_cast<uint32_t>(rows) : 1u << group_log;
+        const uint64_t spans = (facts[0].tile_cols << lane_spread(most, p.logits.tile_cols)) / kTile;
+        ctas = 1;
+        while (ctas < kMaxCluster && spans >= static_cast<uint64_t>(ctas) * 2 * kScoreWarps * 2) ctas *= 2;
+        p.bands = static_cast<uint32_t>((rows + (1u << group_log) - 1) >> group_log);
+        if (group_log == 0 || facts[0].planes * p.bands * ctas >= static_cast<uint64_t>(sm_count())) break;
+    }
+    p.group_log = group_log;
     const uint64_t grid = (facts[0].planes * p.bands + 1) * ctas;
     if (grid > 0x7FFFFFFFull) return fail(IOMB_ERR_UNSUPPORTED, "token_logprobs: too many rows for one launch");
     cudaLaunchConfig_t config{};
