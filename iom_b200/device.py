@@ -587,6 +587,7 @@ class B200Queue:
         self._sequence = 0
         self._records = {}        # sequence -> (event, owners, status cell or None)
         self._failures = {}       # sequence -> exception
+        self._events = []         # completion events of finished operations, to be used again
         self._completed = 0
         self._closed = False
         self._capture = None      # the CapturedSequence being recorded, if any
@@ -628,8 +629,7 @@ class B200Queue:
     def _retire(self, limit: int) -> None:
         """Bounds in-flight work to the configured credit count."""
         while len(self._records) >= limit:
-            oldest = min(self._records)
-            self._finish(oldest)
+            self._finish(next(iter(self._records)))     # (records are in submission order)
 
     def _finish(self, sequence: int) -> None:
         record = self._records.pop(sequence, None)
@@ -639,7 +639,9 @@ class B200Queue:
         if event is None:
             self._stream.synchronize()      # no event could be recorded: drain the stream
         else:
-            event.synchronize()
+            if not event.query():
+                event.synchronize()
+            self._events.append(event)
         if self.faults.take("complete"):
             self._failures[sequence] = DeviceError("injected completion failure")
             return
@@ -653,7 +655,7 @@ class B200Queue:
             return self._submit_captured(launch, owners, status_cell)
         try:
             self._retire(self._device.queue_config.max_in_flight_per_queue)
-            with torch.cuda.device(self._device.torch_device):
+            with torch.cuda.device(self._device.ordinal):
                 if self.faults.take("launch"):
                     raise DeviceError("injected launch failure")
                 status = launch(self._stream.cuda_stream)
@@ -661,7 +663,8 @@ class B200Queue:
                     raise _status_to_exception(status)
                 event = None
                 if not self.faults.take("record"):
-                    event = torch.cuda.Event()
+                    # (an event that was waited for is free again; at most one per credit exists)
+                    event = self._events.pop() if self._events else torch.cuda.Event()
                     event.record(self._stream)
                 pinned = None
                 if status_cell is not None:
@@ -1035,7 +1038,7 @@ class B200Queue:
         for view in views:
             if view is not None:
                 self._check_view(view, what)
-        return [None if view is None else ctypes.byref(view.as_abi()) for view in views]
+        return [None if view is None else view.abi_reference() for view in views]
 
     def sdpa_packed(self, q: TensorView, k: TensorView, v: TensorView, out: TensorView,
                     offsets: int, sequences: int, status: int, scale: Optional[float] = None) -> int:

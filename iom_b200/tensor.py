@@ -9,6 +9,7 @@ std::overflow_error -> OverflowError, std::bad_alloc -> MemoryError.
 """
 from __future__ import annotations
 
+import ctypes
 import enum
 from dataclasses import dataclass
 from typing import Sequence
@@ -165,13 +166,14 @@ class TensorView:
     `storage_nbytes` and `device`.
     """
 
-    __slots__ = ("_owner", "_spec", "_plane_offset", "_plane_strides")
+    __slots__ = ("_owner", "_spec", "_plane_offset", "_plane_strides", "_snapshot")
 
     def __init__(self, owner, spec: TensorSpec, plane_offset: int, plane_strides: Sequence[int]):
         self._owner = owner
         self._spec = spec
         self._plane_offset = int(plane_offset)
         self._plane_strides = tuple(int(s) for s in plane_strides)
+        self._snapshot = None
 
     @property
     def spec(self) -> TensorSpec:
@@ -301,6 +303,13 @@ class TensorView:
         for i, stride in enumerate(self._plane_strides[:MAX_LEADING]):
             view.plane_strides[i] = stride
         return view
+
+    def abi_reference(self):
+        """A pointer to the view's value snapshot, made once (a view never changes, nor does
+        its owner's address); for calls that only read it."""
+        if self._snapshot is None:
+            self._snapshot = ctypes.byref(self.as_abi())
+        return self._snapshot
 
     # Host transfers are provided by the owning device tensor.
     def copy_from_host(self, source, workspace=None) -> None:
