@@ -1,14 +1,16 @@
 // Attention on the tensor cores: the kernel behind iomb_sdpa_packed and iomb_sdpa_tree for head
 // widths that are multiples of 16 up to 128.
 //
-// One CTA works on two tiles, A and B, of 128 score rows each. Per block of 128 tokens and tile
+// One CTA works on two tiles, A and B, of 128 score rows each. Per step of 64 tokens and tile
 //   S = Q K^T          tcgen05.mma, both operands in shared memory, S in tensor memory (FP32)
 //   P = exp2(c S - c m) softmax warpgroup of the tile: one thread per row, S read back from
 //                      tensor memory, P (16-bit) written over S
 //   O += P V           tcgen05.mma, P from tensor memory, V from shared memory, O in tensor memory
 // with the running maximum m and sum l of each row in its thread. O is rescaled only when a
 // row's maximum grows by more than 2^8 (P then stays below 2^8, far from any overflow); the sum
-// takes the unrounded exponentials. While one tile's softmax runs, the other tile's products do.
+// takes the unrounded exponentials. S has two buffers per tile: the scores of the next step are
+// there when the softmax of this one ends, so the exponentials, which bound the kernel (16 a
+// clock and SM), run without a pause.
 //
 // The library's 16x16 tiles feed the matrix instructions without any re-layout: a tile row is 32
 // bytes, so a column of tiles is a K-major operand with 32-byte swizzle and K = 16 (one
@@ -19,8 +21,8 @@
 //   packed   `pack` heads of one key/value head x 128/pack consecutive rows, so that short
 //            sequences share a tile between heads; A and B are neighbouring row blocks
 //   tree     the (head, node) pairs of one key/value head. Up to 128 pairs: both tiles hold the
-//            same rows and take alternate token blocks, joined at the end. More: A and B hold
-//            128 pairs each and share the token blocks
+//            same rows, A takes the first half of every block of 128 tokens and B the second,
+//            joined at the end. More: A and B hold 128 pairs each and share the tokens
 // The tree call cuts the token blocks of all sequences and heads into equal ranges, one per CTA.
 // A row whose blocks lie in several ranges leaves partial (m, l, O) in the workspace and a second
 // kernel joins them, in the order of the ranges.
@@ -29,9 +31,10 @@
 // but also garbage under the mask, which the matrix instruction multiplies by zero) is computed
 // again by attend_row, which reads visible tokens only.
 //
-// Warps: 0-3 softmax of A, 4-7 softmax of B, 8 issues the matrix instructions, 9 the copies (10
-// and 11 fill their warpgroup, which hands registers to the softmax: 2 x 128 x 208 + 128 x 80
-// of the 384 x 168 the CTA starts with).
+// Warps: 0-3 softmax of A, 4-7 softmax of B, 8 issues the matrix instructions, 9 the copies, 10
+// and 11 bring the queries of a tree call's next row set while the last one is worked on. The
+// last four hand registers to the softmax (2 x 128 x 208 + 128 x 80 of the 384 x 168 a CTA
+// starts with).
 // Every wait is bounded; one that gives up ends all roles and is counted.
 #include <cuda.h>
 
@@ -48,7 +51,8 @@ constexpr uint32_t kTileRows = 128;
 constexpr uint32_t kMaxWidth = 128;
 constexpr uint32_t kMaxStages = 8;
 constexpr uint32_t kRingBytes = 128 * 1024;
-constexpr uint32_t kTmemColumns = 512;          // S of A and B: 0, 128; O of A and B: 256, 384
+constexpr uint32_t kStep = 64;                  // tokens per softmax step
+constexpr uint32_t kTmemColumns = 512;          // S of A and B: 2 x 64 at 0, 128; O of A and B: 256, 384
 constexpr uint32_t kMaskWords = kMaxTreeNodes / 32;
 constexpr float kRescale = 8.0f;                // in powers of two
 // Bounds of the waits: about a second, and a quarter of a minute where the other side may be
@@ -67,6 +71,7 @@ struct TcParams {
     // tree
     uint32_t members;           // (head, node) pairs per key/value head
     uint32_t alternate;         // both tiles hold the same rows
+    uint32_t query_buffers;     // one, or two where they fit
     uint32_t pairs;             // tile pairs per key/value head
     uint32_t row_cap;           // rows of one partial
     uint64_t slot_floats;       // floats of one partial: row_cap * (D + 2), a multiple of eight
@@ -107,6 +112,14 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatil
     } while (clock64() - start < limit);
     *stop = 1;
     return false;
+}
+// Whether any of the 256 softmax threads says so; a barrier for them.
+__device__ __forceinline__ bool any_of_softmax(bool mine) {
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred mine, any;\n\tsetp.ne.u32 mine, %1, 0;\n\t"
+                 "barrier.cta.red.or.pred any, 1, 256, mine;\n\tselp.u32 %0, 1, 0, any;\n\t}"
+                 : "=r"(any) : "r"(mine ? 1u : 0u) : "memory");
+    return any != 0;
 }
 // 128 tokens x D of one plane: tile rows [tile_row, tile_row + 8), every tile column.
 __device__ __forceinline__ void copy_block(uint32_t dst, const CUtensorMap* map, uint64_t* bar, uint32_t tile_row,
@@ -164,6 +177,10 @@ __device__ __forceinline__ void tmem_store16(uint32_t address, const uint32_t* r
             : "memory");
 }
 
+__device__ __forceinline__ void store_shared(uint32_t address, uint4 v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(address), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
 // Shared-memory operand with 32-byte swizzle. Groups of eight 32-byte rows lie 256 bytes apart
 // (stride offset); the leading offset is the distance of neighbouring 16-column pieces and only
 // the MN-major operand (V) uses it.
@@ -176,20 +193,29 @@ __device__ __forceinline__ uint32_t product_descriptor(uint32_t format, uint32_t
     return (1u << 4) | (format << 7) | (format << 10) | ((b_mn ? 1u : 0u) << 16) | ((n >> 3) << 17)
             | ((kTileRows >> 4) << 24);
 }
-__device__ __forceinline__ void mma_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t kind, bool accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(kind), "r"(accumulate ? 1u : 0u) : "memory");
+// The warp that issues runs as a whole, on values that are the same in every lane, and one lane's
+// predicate guards each instruction: their operands then stay in uniform registers. (Issued inside
+// a one-lane branch an instruction took 85 cycles, more than many of them compute.)
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t mine;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(mine));
+    return mine;
 }
-__device__ __forceinline__ void mma_tensor(uint32_t d, uint32_t a, uint64_t b, uint32_t kind, bool accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(kind), "r"(accumulate ? 1u : 0u) : "memory");
+__device__ __forceinline__ void mma_shared(uint32_t lane, uint32_t d, uint64_t a, uint64_t b, uint32_t kind, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(kind), "r"(accumulate), "r"(lane) : "memory");
+}
+__device__ __forceinline__ void mma_tensor(uint32_t lane, uint32_t d, uint32_t a, uint64_t b, uint32_t kind, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(kind), "r"(accumulate), "r"(lane) : "memory");
 }
 // The barrier is reached when every matrix instruction issued so far has completed.
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-                 ::"r"(shared_address(bar)) : "memory");
+__device__ __forceinline__ void mma_commit(uint32_t lane, uint64_t* bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+                 ::"r"(shared_address(bar)), "r"(lane) : "memory");
 }
 
 // Packed binary32 pairs: one instruction per two values.
@@ -223,7 +249,8 @@ __device__ __forceinline__ float exp2_fast(float x) {
 struct Piece {
     uint32_t b, kv_head, pair;  // sequence, key/value head, tile pair
     uint32_t first_token;       // multiple of 16: the first block's first row of k and v
-    uint32_t blocks[2];         // per tile; equal in a tree call
+    uint32_t blocks;            // blocks of 128 tokens; none: there are no more pieces
+    uint32_t steps[2];          // per tile, of 64 tokens
     uint32_t end;               // rows of the sequence end here (packed), live rows (tree)
     uint32_t row0;              // packed: first row of tile A
     uint32_t start;             // packed: first row of the sequence; tree: rows before the tree
@@ -257,8 +284,15 @@ __device__ __forceinline__ bool next_piece(const TcParams& p, Walk& w, Piece& ou
     out.kv_head = w.set / p.pairs;
     out.pair = w.set % p.pairs;
     out.first_token = w.block * kKvBlock;
-    out.blocks[0] = out.blocks[1] = take;
+    out.blocks = take;
     out.end = e.length + e.nodes;
+    const uint32_t tokens = min(out.end - out.first_token, take * kKvBlock);
+    if (p.alternate) {
+        out.steps[0] = take;
+        out.steps[1] = tokens - (take - 1) * kKvBlock > kStep ? take : take - 1;
+    } else {
+        out.steps[0] = out.steps[1] = (tokens + kStep - 1) / kStep;
+    }
     out.row0 = 0;
     out.start = e.length;
     out.nodes = e.nodes;
@@ -283,6 +317,7 @@ __device__ __forceinline__ uint64_t warp_sum64(uint64_t v) {
 
 // Range [total * cta / ctas, total * (cta + 1) / ctas) of token blocks.
 __device__ __forceinline__ uint64_t range_begin(uint64_t total, uint32_t cta, uint32_t ctas) {
+    if (total < (1u << 22) && ctas < 1024) return static_cast<uint32_t>(total) * cta / ctas;   // (short division)
     return total * cta / ctas;
 }
 
@@ -371,8 +406,9 @@ __device__ __forceinline__ bool plan_packed(const TcParams& p, uint32_t unit, Pi
     for (uint32_t x = 0; x < 2; ++x) {
         const uint32_t row = out.row0 + x * p.tile_rows;
         const uint32_t last = min(out.end, row + p.tile_rows);      // one behind the tile's last row
-        out.blocks[x] = row < out.end ? (last - out.first_token + kKvBlock - 1) / kKvBlock : 0;
+        out.steps[x] = row < out.end ? (last - out.first_token + kStep - 1) / kStep : 0;
     }
+    out.blocks = (max(out.steps[0], out.steps[1]) + 1) / 2;
     out.nodes = 0;
     out.whole = 1;
     out.slot = 0;
@@ -399,13 +435,16 @@ __device__ __noinline__ void redo_row(const AttnParams& p, uint32_t b, uint32_t 
 
 struct Shared {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t scores[2], weights[2], done[2];    // S written, P written, O complete
-    uint64_t queries, drain;
+    uint64_t scores[2][2], weights[2][2];       // per tile and buffer: S written, P written
+    uint64_t values[2];                         // per tile: O holds one more step
+    uint64_t queries[2], queries_free[2];       // a piece's queries are there; its scores are computed
+    uint64_t piece_free[2];                     // nobody reads the piece any more
+    uint64_t drain;
     uint32_t tmem, stop, run;
-    Piece piece;                                // packed
+    Piece pieces[2];
     Walk walk;                                  // tree
-    float other[2][kTileRows];                  // m and l of tile B (alternate blocks)
-    uint32_t mask[kMaxTreeNodes * kMaskWords];  // ancestors and the node itself
+    float other[2][kTileRows];                  // m and l of tile B (same rows)
+    uint32_t mask[2][kMaxTreeNodes * kMaskWords];       // ancestors and the node itself
     int16_t parent[kMaxTreeNodes];
 };
 
@@ -415,12 +454,13 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                     const __grid_constant__ CUtensorMap v_map) {
     extern __shared__ __align__(1024) unsigned char dynamic[];
     __shared__ Shared sh;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31u;     // (the warp: a uniform value)
     const uint32_t width = p.a.width, slices = width / kTile;
     const uint32_t block_bytes = width * kTileRows * 2;         // a Q tile, a K block, a V block
+    const uint32_t query_bytes = (TREE && p.alternate ? 1u : 2u) * block_bytes;
     // The dynamic part starts behind the static one: round up to the swizzle's alignment.
     const uint32_t q_base = (shared_address(dynamic) + 1023u) & ~1023u;
-    const uint32_t ring = q_base + (TREE && p.alternate ? 1u : 2u) * block_bytes;
+    const uint32_t ring = q_base + p.query_buffers * query_bytes;
     volatile uint32_t* const stop = &sh.stop;
 
     if (warp == 0) {
@@ -435,7 +475,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             bool ok;
             const bool run = plan_packed(p, blockIdx.x, piece, ok);
             if (lane == 0) {
-                sh.piece = piece;
+                sh.pieces[0] = piece;
                 sh.run = run;
                 if (blockIdx.x == 0) *p.a.status = ok ? 0u : 1u;
             }
@@ -450,11 +490,15 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             bar_init(&sh.empty[s], 1);
         }
         for (uint32_t x = 0; x < 2; ++x) {
-            bar_init(&sh.scores[x], 1);
-            bar_init(&sh.weights[x], 4);
-            bar_init(&sh.done[x], 1);
+            for (uint32_t i = 0; i < 2; ++i) {
+                bar_init(&sh.scores[x][i], 1);
+                bar_init(&sh.weights[x][i], 4);
+            }
+            bar_init(&sh.values[x], 1);
+            bar_init(&sh.queries[x], TREE ? 2 : kSoftmaxWarps);
+            bar_init(&sh.queries_free[x], 1);
+            bar_init(&sh.piece_free[x], kSoftmaxWarps);
         }
-        bar_init(&sh.queries, kSoftmaxWarps);
         bar_init(&sh.drain, 1);
         sh.stop = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -465,7 +509,6 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
     if constexpr (TREE) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem = sh.tmem;
     const bool run = sh.run != 0;
-
     if (warp < kSoftmaxWarps) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
 
@@ -475,12 +518,18 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
         const uint32_t lanes = (warp & 3u) << 21;               // this warp's 32 tensor memory lanes
         const uint32_t s_at = tmem + lanes + x * 128, o_at = tmem + lanes + 256 + x * 128;
         const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
-        uint32_t steps_done = 0, pieces_done = 0;               // completed phases of this tile's barriers
-        Walk walk = sh.walk;
-        Piece piece = sh.piece;
-        bool go = TREE ? next_piece(p, walk, piece) : true;
-        while (go) {
-            const uint32_t n = TREE && p.alternate ? (piece.blocks[0] + 1 - x) / 2 : piece.blocks[x];
+        uint32_t steps_done = 0;                                // of this tile, over all pieces
+        bool alive = true;
+        for (uint32_t turn = 0; ; ++turn) {
+            const uint32_t buffer = turn & 1u;
+            if constexpr (TREE) {
+                alive = __all_sync(0xffffffffu, bar_wait(&sh.queries[buffer], (turn / 2) & 1u, stop, kLongWaitCycles));
+                if (p.alternate) alive = !any_of_softmax(!alive);       // (one answer: barriers follow)
+                if (!alive) break;
+            }
+            const Piece& piece = sh.pieces[TREE ? buffer : 0];
+            if (piece.blocks == 0) break;
+            const uint32_t n = piece.steps[x], start = piece.start;
             // This thread's row.
             uint32_t head, row;
             bool valid;
@@ -495,81 +544,62 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                 valid = row < piece.end;
             }
             const bool busy = __any_sync(0xffffffffu, valid) && n != 0;
-            if constexpr (TREE) {
-                // Ancestor masks, when the piece reaches the tree; nobody still reads the last piece's.
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-                if (p.a.parents != nullptr && piece.first_token + piece.blocks[0] * kKvBlock > piece.start) {
-                    const int32_t* parents = p.a.parents + static_cast<uint64_t>(piece.b) * p.a.rows;
-                    for (uint32_t i = threadIdx.x; i < piece.nodes; i += 256) {
-                        sh.parent[i] = static_cast<int16_t>(max(-1, tree_parent(parents, static_cast<int32_t>(i))));
-                    }
-                    asm volatile("bar.sync 1, 256;" ::: "memory");
-                    for (uint32_t i = threadIdx.x; i < piece.nodes; i += 256) {
-                        uint32_t* words = sh.mask + i * kMaskWords;
-                        for (uint32_t w = 0; w < kMaskWords; ++w) words[w] = 0;
-                        for (int32_t at = static_cast<int32_t>(i); at >= 0; at = sh.parent[at]) {
-                            words[at / 32] |= 1u << (at % 32);
+            if constexpr (!TREE) {
+                // Q: 32 bytes of a tile row at a time, into the swizzled K-major operand.
+                if (n != 0) {
+                    const uint64_t plane = attn_plane(p.a.q, piece.b, head);
+                    const uint32_t dst = q_base + x * block_bytes + m * 32;
+                    const uint32_t flip = ((m >> 2) & 1u) * 16;
+                    for (uint32_t c = 0; c < slices; ++c) {
+                        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+                        if (valid) {
+                            const uint4* src = reinterpret_cast<const uint4*>(attn_piece(p.a.q, plane, row, c));
+                            lo = src[0];
+                            hi = src[1];
                         }
+                        store_shared(dst + c * 4096 + flip, lo);
+                        store_shared(dst + c * 4096 + (16 - flip), hi);
                     }
-                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
+                __syncwarp();
+                if (lane == 0) bar_arrive(&sh.queries[0]);
             }
-            // Q: 32 bytes of a tile row per step, into the swizzled K-major operand.
-            if (!(TREE && p.alternate && x == 1) && n != 0) {
-                const uint64_t plane = attn_plane(p.a.q, piece.b, head);
-                const uint32_t dst = q_base + x * block_bytes + m * 32;
-                const uint32_t flip = ((m >> 2) & 1u) * 16;
-                for (uint32_t c = 0; c < slices; ++c) {
-                    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-                    if (valid) {
-                        const uint4* src = reinterpret_cast<const uint4*>(attn_piece(p.a.q, plane, row, c));
-                        lo = src[0];
-                        hi = src[1];
-                    }
-                    const uint32_t at = dst + c * 4096;
-                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at + flip), "r"(lo.x), "r"(lo.y), "r"(lo.z),
-                                 "r"(lo.w) : "memory");
-                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at + (16 - flip)), "r"(hi.x), "r"(hi.y),
-                                 "r"(hi.z), "r"(hi.w) : "memory");
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            }
-            __syncwarp();
-            if (lane == 0) bar_arrive(&sh.queries);
 
-            float top = __int_as_float(0xFF800000), sum = 0.0f;     // running maximum (of S) and sum
-            bool alive = true;
-            for (uint32_t step = 0; step < n; ++step) {
+            const float kNone = __int_as_float(0xFF800000);
+            float top = kNone, sum = 0.0f;                      // running maximum (of S) and sum
+            const uint32_t first = piece.first_token + (TREE && p.alternate ? x * kStep : 0u);
+            const uint32_t stride = TREE && p.alternate ? kKvBlock : kStep;
+            // Tokens from here on may be hidden from some row of the tile.
+            const uint32_t clear = TREE ? start : piece.row0 + x * p.tile_rows + 1;
+            for (uint32_t step = 0; step < n; ++step, ++steps_done) {
+                const uint32_t buf = steps_done & 1u, phase = (steps_done >> 1) & 1u;
                 // (one answer per warp)
-                alive = __all_sync(0xffffffffu, bar_wait(&sh.scores[x], steps_done & 1u, stop));
+                alive = __all_sync(0xffffffffu, bar_wait(&sh.scores[x][buf], phase, stop));
                 if (!alive) break;
-                ++steps_done;
                 tmem_after_sync();
                 if (busy) {
-                    uint32_t s[128];
-                    tmem_load32(s_at, s);
-                    tmem_load32(s_at + 32, s + 32);
-                    tmem_load32(s_at + 64, s + 64);
-                    tmem_load32(s_at + 96, s + 96);
-                    const uint32_t block = TREE && p.alternate ? 2 * step + x : step;
-                    const uint32_t token = piece.first_token + block * kKvBlock;
-                    const bool masked = TREE ? token + kKvBlock > piece.start
-                                             : token < piece.start || token + kKvBlock > piece.row0 + x * p.tile_rows + 1;
+                    uint32_t s[kStep];
+                    const uint32_t at = s_at + buf * kStep;
+                    tmem_load32(at, s);
+                    tmem_load32(at + 32, s + 32);
+                    const uint32_t token = first + step * stride;
+                    const bool masked = token + kStep > clear || (!TREE && token < start);
                     tmem_wait_load();
                     if (masked) {
-                        uint32_t see[4];
+                        uint32_t see[kStep / 32];
 #pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            const int32_t first = static_cast<int32_t>(token) + 32 * w;
+                        for (int w = 0; w < static_cast<int>(kStep / 32); ++w) {
+                            const int32_t from = static_cast<int32_t>(token) + 32 * w;
                             if constexpr (!TREE) {
-                                see[w] = range_word(static_cast<int32_t>(piece.start) - first, static_cast<int32_t>(row) - first);
+                                see[w] = range_word(static_cast<int32_t>(start) - from, static_cast<int32_t>(row) - from);
                             } else if (p.a.parents == nullptr) {
-                                see[w] = range_word(0, static_cast<int32_t>(piece.start + row) - first);
+                                see[w] = range_word(0, static_cast<int32_t>(start + row) - from);
                             } else {
-                                see[w] = range_word(0, static_cast<int32_t>(piece.start) - 1 - first);
-                                const int32_t rel = first - static_cast<int32_t>(piece.start);
+                                see[w] = range_word(0, static_cast<int32_t>(start) - 1 - from);
+                                const int32_t rel = from - static_cast<int32_t>(start);
                                 if (valid && rel > -32 && rel < static_cast<int32_t>(kMaxTreeNodes)) {
-                                    const uint32_t* words = sh.mask + row * kMaskWords;
+                                    const uint32_t* words = sh.mask[buffer] + row * kMaskWords;
                                     if (rel < 0) {
                                         see[w] |= words[0] << -rel;
                                     } else {
@@ -581,7 +611,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                             if (!valid) see[w] = 0;
                         }
 #pragma unroll
-                        for (int c = 0; c < 128; ++c) {
+                        for (int c = 0; c < static_cast<int>(kStep); ++c) {
                             if (!((see[c / 32] >> (c % 32)) & 1u)) s[c] = 0xFF800000u;
                         }
                     }
@@ -589,17 +619,21 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
 #pragma unroll
                     for (int i = 0; i < 4; ++i) best[i] = fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 4]));
 #pragma unroll
-                    for (int c = 8; c < 128; c += 8) {
+                    for (int c = 8; c < static_cast<int>(kStep); c += 8) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             best[i] = fmaxf(fmaxf(best[i], __uint_as_float(s[c + i])), __uint_as_float(s[c + i + 4]));
                         }
                     }
                     const float high = fmaxf(top, fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])));
-                    // The first block, or a maximum that grew beyond what P may: a new reference.
-                    const bool fresh = top == __int_as_float(0xFF800000);
+                    // The first tokens seen, or a maximum that grew beyond what P may: a new reference.
+                    const bool fresh = top == kNone;
                     const bool grow = !fresh && (high - top) * p.scale_log2 > kRescale;
-                    if (__any_sync(0xffffffffu, grow) && step != 0) {
+                    if (__any_sync(0xffffffffu, grow)) {
+                        // (not the first step: O holds the steps before this one once they are done)
+                        alive = __all_sync(0xffffffffu, bar_wait(&sh.values[x], (steps_done - 1) & 1u, stop));
+                        if (!alive) break;
+                        tmem_after_sync();
                         const float factor = grow ? exp2_fast((top - high) * p.scale_log2) : 1.0f;
                         sum *= factor;
                         for (uint32_t c = 0; c < slices; ++c) {
@@ -612,11 +646,11 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                         }
                     }
                     if (fresh || grow) top = high;
-                    const float shift = top == __int_as_float(0xFF800000) ? 0.0f : -(top * p.scale_log2);
+                    const float shift = top == kNone ? 0.0f : -(top * p.scale_log2);
                     const uint64_t shift2 = pair(shift, shift);
                     uint64_t sums[4] = {0, 0, 0, 0};
 #pragma unroll
-                    for (int c = 0; c < 128; c += 2) {
+                    for (int c = 0; c < static_cast<int>(kStep); c += 2) {
                         float e0, e1;
                         unpair(fma2(pair(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), scale2, shift2), e0, e1);
                         e0 = exp2_fast(e0);
@@ -624,8 +658,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                         sums[(c / 2) % 4] = add2(sums[(c / 2) % 4], pair(e0, e1));
                         s[c / 2] = Leaf::pack(e0, e1);
                     }
-                    tmem_store32(s_at, s);
-                    tmem_store32(s_at + 32, s + 32);
+                    tmem_store32(at, s);
                     float a, b;
                     unpair(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])), a, b);
                     sum += a + b;
@@ -633,16 +666,19 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                 }
                 tmem_before_sync();
                 __syncwarp();
-                if (lane == 0) bar_arrive(&sh.weights[x]);
+                if (lane == 0) bar_arrive(&sh.weights[x][buf]);
             }
             if (alive && n != 0) {
-                alive = __all_sync(0xffffffffu, bar_wait(&sh.done[x], pieces_done & 1u, stop));
-                ++pieces_done;
+                // The last two steps, one after the other: a wait tells a phase from the one before
+                // it only, and the scores of the last step say no more than that the step three
+                // back is done.
+                if (n > 1) alive = bar_wait(&sh.values[x], (steps_done - 2) & 1u, stop);
+                alive = __all_sync(0xffffffffu, alive && bar_wait(&sh.values[x], (steps_done - 1) & 1u, stop));
                 tmem_after_sync();
             }
             // ---- results ---------------------------------------------------------------------------
             const bool join = TREE && p.alternate;
-            const bool second = join && piece.blocks[0] > 1;       // tile B holds part of the sum
+            const bool second = join && piece.steps[1] != 0;        // tile B holds part of the sum
             float mine = 1.0f, its = 0.0f;                          // factors of the two tiles' O
             if (join) {
                 if (x == 1) {
@@ -660,184 +696,168 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                 }
             }
             if (alive && busy && !(join && x == 1)) {
-                const uint32_t b_at = o_at + 128;
-                if (!TREE || piece.whole) {
-                    const float inverse = 1.0f / sum;
-                    bool bad = !(sum > 0.0f && sum <= 3.0e38f);
-                    const uint64_t plane = attn_plane(p.a.out, piece.b, 0);
-                    const uint32_t column = head * slices;
-                    for (uint32_t c = 0; c < slices; ++c) {
-                        uint32_t o[16], o2[16];
-                        tmem_load16(o_at + c * 16, o);
-                        if (second) tmem_load16(b_at + c * 16, o2);
-                        tmem_wait_load();
-                        uint32_t packed[8];
+                const bool whole = !TREE || piece.whole;
+                const float inverse = whole ? 1.0f / sum : 1.0f;
+                bool bad = !(sum > 0.0f && sum <= 3.0e38f);
+                const uint64_t plane = attn_plane(p.a.out, piece.b, 0);
+                const uint32_t column = head * slices, local = (TREE && !p.alternate ? x * 128 : 0u) + m;
+                float* const slot = p.partial + static_cast<uint64_t>(blockIdx.x * 2 + piece.slot) * p.slot_floats;
+                for (uint32_t c = 0; c < slices; c += 2) {
+                    // (32 columns at a time; those behind the head's width are not used)
+                    uint32_t o[32], o2[32];
+                    tmem_load32(o_at + c * 16, o);
+                    if (second) tmem_load32(o_at + 128 + c * 16, o2);
+                    tmem_wait_load();
+                    if (second) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            float v = __uint_as_float(o[i]);
-                            if (second) {
-                                v = mine == 0.0f ? 0.0f : v * mine;
-                                if (its != 0.0f) v = __fmaf_rn(__uint_as_float(o2[i]), its, v);
-                            }
-                            v *= inverse;
-                            bad = bad || !(fabsf(v) <= 3.4028234e38f);
+                        for (int i = 0; i < 32; ++i) {
+                            float v = mine == 0.0f ? 0.0f : __uint_as_float(o[i]) * mine;
+                            if (its != 0.0f) v = __fmaf_rn(__uint_as_float(o2[i]), its, v);
                             o[i] = __float_as_uint(v);
                         }
+                    }
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            packed[i] = canonical_pair<Leaf>(Leaf::pack(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])));
-                        }
-                        if (valid) {
-                            store_u8_stream(attn_out_piece(p.a.out, plane, row, column + c),
-                                            make_uint4(packed[0], packed[1], packed[2], packed[3]),
-                                            make_uint4(packed[4], packed[5], packed[6], packed[7]));
+                    for (int half = 0; half < 2; ++half) {
+                        if (c + half >= slices) break;
+                        uint32_t* const part = o + 16 * half;
+                        if (whole) {
+                            uint32_t packed[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const float lo = __uint_as_float(part[2 * i]) * inverse, hi = __uint_as_float(part[2 * i + 1]) * inverse;
+                                bad = bad || !(fabsf(lo) <= 3.4028234e38f) || !(fabsf(hi) <= 3.4028234e38f);
+                                packed[i] = canonical_pair<Leaf>(Leaf::pack(lo, hi));
+                            }
+                            if (valid) {
+                                store_u8_stream(attn_out_piece(p.a.out, plane, row, column + c + half),
+                                                make_uint4(packed[0], packed[1], packed[2], packed[3]),
+                                                make_uint4(packed[4], packed[5], packed[6], packed[7]));
+                            }
+                        } else if (valid) {
+                            uint4* to = reinterpret_cast<uint4*>(slot + static_cast<uint64_t>(local) * width + (c + half) * 16);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                to[i] = make_uint4(part[4 * i], part[4 * i + 1], part[4 * i + 2], part[4 * i + 3]);
+                            }
                         }
                     }
+                }
+                if (whole) {
                     uint32_t again = __ballot_sync(0xffffffffu, bad && valid);
                     while (again != 0) {
                         const int who = __ffs(again) - 1;
                         again &= again - 1;
                         __syncwarp();
                         redo_row<Leaf, TREE>(p.a, piece.b, __shfl_sync(0xffffffffu, head, who),
-                                             __shfl_sync(0xffffffffu, row, who), piece.start);
+                                             __shfl_sync(0xffffffffu, row, who), start);
                     }
-                } else if constexpr (TREE) {
-                    const uint32_t local = (p.alternate ? 0u : x * 128) + m;
-                    float* slot = p.partial + static_cast<uint64_t>(blockIdx.x * 2 + piece.slot) * p.slot_floats;
-                    for (uint32_t c = 0; c < slices; ++c) {
-                        uint32_t o[16], o2[16];
-                        tmem_load16(o_at + c * 16, o);
-                        if (second) tmem_load16(b_at + c * 16, o2);
-                        tmem_wait_load();
-                        if (second) {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                float v = mine == 0.0f ? 0.0f : __uint_as_float(o[i]) * mine;
-                                if (its != 0.0f) v = __fmaf_rn(__uint_as_float(o2[i]), its, v);
-                                o[i] = __float_as_uint(v);
-                            }
-                        }
-                        if (valid) {
-                            uint4* to = reinterpret_cast<uint4*>(slot + static_cast<uint64_t>(local) * width + c * 16);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) to[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-                        }
-                    }
-                    if (valid) {
-                        slot[static_cast<uint64_t>(p.row_cap) * width + local] = top;
-                        slot[static_cast<uint64_t>(p.row_cap) * (width + 1) + local] = sum;
-                    }
+                } else if (valid) {
+                    slot[static_cast<uint64_t>(p.row_cap) * width + local] = top;
+                    slot[static_cast<uint64_t>(p.row_cap) * (width + 1) + local] = sum;
                 }
             }
             if constexpr (!TREE) break;
-            // Both tiles' results are out of tensor memory; one give-up ends both.
             tmem_before_sync();
-            uint32_t over;
-            asm volatile("{\n\t.reg .pred mine, any;\n\tsetp.ne.u32 mine, %1, 0;\n\t"
-                         "barrier.cta.red.or.pred any, 1, 256, mine;\n\tselp.u32 %0, 1, 0, any;\n\t}"
-                         : "=r"(over) : "r"(alive && *stop == 0 ? 0u : 1u) : "memory");
-            if (over != 0) break;
-            go = next_piece(p, walk, piece);
+            if (join) {
+                // Both tiles' results are out of tensor memory; one give-up ends both.
+                alive = !any_of_softmax(!alive || *stop != 0);
+            }
+            if (!alive) break;
+            __syncwarp();
+            if (lane == 0) bar_arrive(&sh.piece_free[buffer]);
         }
     } else if (run && warp == 8) {
-        // ---- matrix instructions, one thread -----------------------------------------------------------
-        if (lane == 0) {
-            const uint32_t kind_s = product_descriptor(Leaf::kFormat, kKvBlock, false);
-            const uint32_t kind_o = product_descriptor(Leaf::kFormat, width, true);
-            uint32_t taken = 0;             // ring slots consumed
-            uint32_t weights_seen[2] = {0, 0};
-            uint32_t pieces = 0;
-            bool alive = true;
-            Walk walk = sh.walk;
-            Piece piece = sh.piece;
-            bool go = TREE ? next_piece(p, walk, piece) : true;
-            auto wait_slot = [&](uint32_t& at) {
-                const uint32_t slot = taken % p.stages;
-                alive = alive && bar_wait(&sh.full[slot], (taken / p.stages) & 1u, stop);
-                ++taken;
+        // ---- matrix instructions ---------------------------------------------------------------------
+        const uint32_t leader = elect_lane();
+        const uint32_t kind_s = product_descriptor(Leaf::kFormat, kStep, false);
+        const uint32_t kind_o = product_descriptor(Leaf::kFormat, width, true);
+        const bool same_rows = TREE && p.alternate;
+        const uint32_t columns = __shfl_sync(0xffffffffu, tmem, 0);
+        uint32_t slot = 0, round = 0;               // next ring slot, and its phase
+        uint32_t scored[2] = {0, 0}, weighed[2] = {0, 0};       // steps of each tile, over all pieces
+        bool alive = true;
+        auto reach = [&](uint64_t* bar, uint32_t phase, long long limit) {
+            alive = __all_sync(0xffffffffu, bar_wait(bar, phase & 1u, stop, limit));
+        };
+        for (uint32_t turn = 0; ; ++turn) {
+            const uint32_t buffer = TREE ? turn & 1u : 0u;
+            reach(&sh.queries[buffer], turn / 2, kLongWaitCycles);
+            if (!alive) break;
+            tmem_after_sync();
+            const uint32_t blocks = __shfl_sync(0xffffffffu, sh.pieces[buffer].blocks, 0);
+            if (blocks == 0) break;
+            const uint32_t steps0 = __shfl_sync(0xffffffffu, sh.pieces[buffer].steps[0], 0);
+            const uint32_t steps1 = __shfl_sync(0xffffffffu, sh.pieces[buffer].steps[1], 0);
+            const uint32_t most = max(steps0, steps1);
+            const uint32_t place = TREE && p.query_buffers == 2 ? buffer : 0u;
+            const uint64_t queries = operand_descriptor(q_base + place * query_bytes, 0);
+            uint32_t k_have = 0, v_have = 0, k_slot = 0, v_slot = 0;
+            auto take = [&](uint32_t& have, uint32_t& at) {
+                reach(&sh.full[slot], round, kWaitCycles);
                 at = slot;
+                ++have;
+                if (++slot == p.stages) { slot = 0; ++round; }
             };
-            auto score = [&](uint32_t x, uint32_t slot) {       // S of tile x = Q K^T
-                const uint32_t q = q_base + (TREE && p.alternate ? 0u : x) * block_bytes;
-                const uint32_t k = ring + slot * block_bytes;
+            // S of tile x for step j = Q K^T; the caller has the step's keys.
+            auto score = [&](uint32_t x, uint32_t j) {
+                const uint32_t half = same_rows ? x : j & 1u, buf = scored[x]++ & 1u;
+                uint64_t k = operand_descriptor(ring + k_slot * block_bytes + half * (kStep * 32), 0);
+                uint64_t rows = queries + (same_rows ? 0u : x * (block_bytes >> 4));
                 for (uint32_t c = 0; c < slices; ++c) {
-                    mma_shared(tmem + x * 128, operand_descriptor(q + c * 4096, 0), operand_descriptor(k + c * 4096, 0),
-                               kind_s, c != 0);
+                    mma_shared(leader, columns + x * 128 + buf * kStep, rows, k, kind_s, c);
+                    rows += 4096 >> 4;
+                    k += 4096 >> 4;
                 }
-                mma_commit(&sh.scores[x]);
+                mma_commit(leader, &sh.scores[x][buf]);
             };
-            auto values = [&](uint32_t x, uint32_t slot, bool first) {      // O of tile x += P V
-                alive = alive && bar_wait(&sh.weights[x], weights_seen[x]++ & 1u, stop);
-                tmem_after_sync();
-                if (!alive) return;
-                const uint32_t v = ring + slot * block_bytes;
-                for (uint32_t t = 0; t < kKvBlock / kTile; ++t) {
-                    mma_tensor(tmem + 256 + x * 128, tmem + x * 128 + t * 8, operand_descriptor(v + t * 512, 4096), kind_o,
-                               !(first && t == 0));
-                }
-            };
-            while (go && alive) {
-                alive = bar_wait(&sh.queries, pieces++ & 1u, stop, kLongWaitCycles);
-                tmem_after_sync();
+            // A block of keys (or values) is free when its last step is issued.
+            auto last_of_block = [&](uint32_t j) { return same_rows || (j & 1u) || j + 1 == most; };
+            for (uint32_t j = 0; j < 2 && j < most; ++j) {
+                if (k_have <= (same_rows ? j : 0u)) take(k_have, k_slot);
                 if (!alive) break;
-                if (TREE && p.alternate) {
-                    const uint32_t n = piece.blocks[0];
-                    uint32_t slot = 0;
-                    for (uint32_t i = 0; i < 2 && i < n && alive; ++i) {
-                        wait_slot(slot);
-                        if (!alive) break;
-                        score(i, slot);
-                        mma_commit(&sh.empty[slot]);
+                if (j < steps0) score(0, j);
+                if (j < steps1) score(1, j);
+                if (last_of_block(j)) mma_commit(leader, &sh.empty[k_slot]);
+                if (TREE && j + 1 == most) mma_commit(leader, &sh.queries_free[place]);
+            }
+            for (uint32_t j = 0; j < most && alive; ++j) {
+                const uint32_t next = j + 2, next_block = same_rows ? next : next >> 1;
+                if (v_have <= (same_rows ? j : j >> 1)) take(v_have, v_slot);
+                if (!alive) break;
+#pragma unroll
+                for (uint32_t x = 0; x < 2; ++x) {
+                    const uint32_t steps = x == 0 ? steps0 : steps1;
+                    if (j >= steps || !alive) continue;
+                    const uint32_t half = same_rows ? x : j & 1u, buf = weighed[x] & 1u, phase = weighed[x] >> 1;
+                    ++weighed[x];
+                    reach(&sh.weights[x][buf], phase, kWaitCycles);
+                    if (!alive) continue;
+                    tmem_after_sync();
+                    const uint64_t v = operand_descriptor(ring + v_slot * block_bytes + half * (kStep / kTile * 512), 4096);
+#pragma unroll
+                    for (uint32_t t = 0; t < kStep / kTile; ++t) {
+                        mma_tensor(leader, columns + 256 + x * 128, columns + x * 128 + buf * kStep + t * 8,
+                                   v + t * (512 >> 4), kind_o, j + t);
                     }
-                    for (uint32_t i = 0; i < n && alive; ++i) {
-                        const uint32_t x = i & 1u;
-                        wait_slot(slot);
-                        if (!alive) break;
-                        values(x, slot, i < 2);
-                        if (!alive) break;
-                        mma_commit(&sh.empty[slot]);
-                        if (i + 2 >= n) {
-                            mma_commit(&sh.done[x]);
-                        } else {
-                            wait_slot(slot);
-                            if (!alive) break;
-                            score(x, slot);
-                            mma_commit(&sh.empty[slot]);
-                        }
-                    }
-                } else {
-                    const uint32_t n = max(piece.blocks[0], piece.blocks[1]);
-                    uint32_t k_slot = 0, v_slot = 0;
-                    wait_slot(k_slot);
-                    if (!alive) break;
-                    for (uint32_t x = 0; x < 2; ++x) {
-                        if (piece.blocks[x] != 0) score(x, k_slot);
-                    }
-                    mma_commit(&sh.empty[k_slot]);
-                    for (uint32_t i = 0; i < n && alive; ++i) {
-                        wait_slot(v_slot);
-                        if (i + 1 < n) wait_slot(k_slot);
-                        if (!alive) break;
-                        for (uint32_t x = 0; x < 2; ++x) {
-                            if (i >= piece.blocks[x]) continue;
-                            values(x, v_slot, i == 0);
-                            if (!alive) break;
-                            if (i + 1 < piece.blocks[x]) score(x, k_slot);
-                            else mma_commit(&sh.done[x]);
-                        }
-                        if (!alive) break;
-                        mma_commit(&sh.empty[v_slot]);
-                        if (i + 1 < n) mma_commit(&sh.empty[k_slot]);
+                    mma_commit(leader, &sh.values[x]);
+                    if (next < steps) {
+                        // (the keys two steps on come behind these values: the order of the copies)
+                        if (k_have <= next_block) take(k_have, k_slot);
+                        if (alive) score(x, next);
                     }
                 }
-                go = TREE ? next_piece(p, walk, piece) : false;
+                if (!alive) break;
+                if (last_of_block(j)) mma_commit(leader, &sh.empty[v_slot]);
+                if (next < most && last_of_block(next)) mma_commit(leader, &sh.empty[k_slot]);
+                if (TREE && next + 1 == most) mma_commit(leader, &sh.queries_free[place]);
             }
-            if (!alive) {
-                // Instructions still in flight end before the tensor memory is given back.
-                mma_commit(&sh.drain);
-                const long long start = clock64();
-                while (!bar_test(&sh.drain, 0) && clock64() - start < kWaitCycles) {}
-            }
+            if (!TREE || !alive) break;
+        }
+        if (!alive) {
+            // Instructions still in flight end before the tensor memory is given back.
+            mma_commit(leader, &sh.drain);
+            const long long start = clock64();
+            while (!bar_test(&sh.drain, 0) && clock64() - start < kWaitCycles) {}
         }
         __syncwarp();
     } else if (run && warp == 9) {
@@ -846,7 +866,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             uint32_t issued = 0;
             bool alive = true;
             Walk walk = sh.walk;
-            Piece piece = sh.piece;
+            Piece piece = sh.pieces[0];
             bool go = TREE ? next_piece(p, walk, piece) : true;
             while (go && alive) {
                 const uint32_t k_plane = static_cast<uint32_t>(attn_plane(p.a.k, piece.b, piece.kv_head));
@@ -854,26 +874,22 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                 const uint32_t first = piece.first_token / kTile;
                 auto fetch = [&](bool keys, uint32_t block) {
                     const uint32_t slot = issued % p.stages;
-                    if (issued >= p.stages) alive = alive && bar_wait(&sh.empty[slot], (issued / p.stages - 1) & 1u, stop, kLongWaitCycles);
+                    if (issued >= p.stages) {
+                        alive = alive && bar_wait(&sh.empty[slot], (issued / p.stages - 1) & 1u, stop, kLongWaitCycles);
+                    }
                     if (!alive) return;
                     bar_expect(&sh.full[slot], block_bytes);
                     copy_block(ring + slot * block_bytes, keys ? &k_map : &v_map, &sh.full[slot],
                                first + block * (kKvBlock / kTile), keys ? k_plane : v_plane);
                     ++issued;
                 };
-                const uint32_t n = max(piece.blocks[0], piece.blocks[1]);
-                if (TREE && p.alternate) {
-                    // In the order the products take them: two key blocks ahead of the values.
-                    for (uint32_t i = 0; i < 2 && i < n && alive; ++i) fetch(true, i);
-                    for (uint32_t i = 0; i < n && alive; ++i) {
-                        fetch(false, i);
-                        if (i + 2 < n && alive) fetch(true, i + 2);
-                    }
-                } else {
-                    for (uint32_t i = 0; i < n && alive; ++i) {
-                        fetch(true, i);
-                        if (alive) fetch(false, i);
-                    }
+                const uint32_t n = piece.blocks;
+                // In the order the products take them: the keys of two steps ahead of the values.
+                const uint32_t ahead = TREE && p.alternate ? 2 : 1;
+                for (uint32_t i = 0; i < ahead && i < n && alive; ++i) fetch(true, i);
+                for (uint32_t i = 0; i < n && alive; ++i) {
+                    fetch(false, i);
+                    if (i + ahead < n && alive) fetch(true, i + ahead);
                 }
                 go = TREE ? next_piece(p, walk, piece) : false;
             }
@@ -889,6 +905,70 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             }
         }
         __syncwarp();
+    } else if (TREE && run) {
+        // ---- queries, pieces and ancestor masks, two warps -----------------------------------------------
+        if constexpr (TREE) {
+            const uint32_t me = threadIdx.x - 10 * 32;
+            Walk walk = sh.walk;
+            Piece piece;
+            bool alive = true;
+            for (uint32_t turn = 0; alive; ++turn) {
+                const uint32_t buffer = turn & 1u;
+                const bool go = next_piece(p, walk, piece);
+                if (!go) piece.blocks = 0;
+                // The piece two turns back is out of use, and the queries that lie where these go.
+                if (turn >= 2) alive = bar_wait(&sh.piece_free[buffer], (turn / 2 - 1) & 1u, stop, kLongWaitCycles);
+                const uint32_t place = p.query_buffers == 2 ? buffer : 0u;
+                const uint32_t used = p.query_buffers == 2 ? turn / 2 : turn;      // times the place was filled
+                if (go && used > 0) alive = alive && bar_wait(&sh.queries_free[place], (used - 1) & 1u, stop, kLongWaitCycles);
+                // (both warps go on or both give up)
+                uint32_t over;
+                asm volatile("{\n\t.reg .pred mine, any;\n\tsetp.ne.u32 mine, %1, 0;\n\t"
+                             "barrier.cta.red.or.pred any, 2, 64, mine;\n\tselp.u32 %0, 1, 0, any;\n\t}"
+                             : "=r"(over) : "r"(alive ? 0u : 1u) : "memory");
+                alive = over == 0;
+                if (!alive) break;
+                if (me == 0) sh.pieces[buffer] = piece;
+                if (go) {
+                    if (p.a.parents != nullptr && piece.first_token + piece.blocks * kKvBlock > piece.start) {
+                        const int32_t* parents = p.a.parents + static_cast<uint64_t>(piece.b) * p.a.rows;
+                        for (uint32_t i = me; i < piece.nodes; i += 64) {
+                            sh.parent[i] = static_cast<int16_t>(max(-1, tree_parent(parents, static_cast<int32_t>(i))));
+                        }
+                        asm volatile("bar.sync 2, 64;" ::: "memory");
+                        for (uint32_t i = me; i < piece.nodes; i += 64) {
+                            uint32_t* words = sh.mask[buffer] + i * kMaskWords;
+                            for (uint32_t w = 0; w < kMaskWords; ++w) words[w] = 0;
+                            for (int32_t at = static_cast<int32_t>(i); at >= 0; at = sh.parent[at]) {
+                                words[at / 32] |= 1u << (at % 32);
+                            }
+                        }
+                    }
+                    // Rows of the set, 32 bytes of a tile row at a time; what the rows behind them
+                    // hold reaches only results nobody stores.
+                    const uint32_t offset = piece.pair * 256;
+                    const uint32_t rows = min(p.alternate ? kTileRows : 2 * kTileRows, p.members - offset);
+                    const uint32_t base = q_base + place * query_bytes;
+                    for (uint32_t c = 0; c < slices; ++c) {
+                        for (uint32_t r = me; r < rows; r += 64) {
+                            const uint32_t member = offset + r;
+                            const uint32_t head = piece.kv_head * p.a.group + member / p.a.rows;
+                            const uint4* src = reinterpret_cast<const uint4*>(
+                                    attn_piece(p.a.q, attn_plane(p.a.q, piece.b, head), member % p.a.rows, c));
+                            const uint4 lo = src[0], hi = src[1];
+                            const uint32_t m = r % kTileRows, flip = ((m >> 2) & 1u) * 16;
+                            const uint32_t to = base + (r / kTileRows) * block_bytes + c * 4096 + m * 32;
+                            store_shared(to + flip, lo);
+                            store_shared(to + (16 - flip), hi);
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                asm volatile("bar.sync 2, 64;" ::: "memory");
+                if (lane == 0) bar_arrive(&sh.queries[buffer]);
+                if (!go) break;
+            }
+        }
     }
     if constexpr (TREE) {
         // (behind the copies, beside the last products)
@@ -941,7 +1021,8 @@ attention_join_kernel(const __grid_constant__ TcParams p, uint32_t ctas) {
     const uint64_t first = before * sets + static_cast<uint64_t>(set) * blocks, end = first + blocks;
     // The ranges that hold block `first` and block `end - 1`.
     auto owner = [&](uint64_t block) {
-        uint32_t c = static_cast<uint32_t>(block * ctas / total);
+        uint32_t c = static_cast<uint32_t>(total < (1u << 22) && ctas < 1024
+                ? static_cast<uint32_t>(block) * ctas / static_cast<uint32_t>(total) : block * ctas / total);
         while (c + 1 < ctas && range_begin(total, c + 1, ctas) <= block) ++c;
         while (c > 0 && range_begin(total, c, ctas) > block) --c;
         return c;
@@ -955,39 +1036,50 @@ attention_join_kernel(const __grid_constant__ TcParams p, uint32_t ctas) {
         const uint32_t member = offset + r, node = member % p.a.rows;
         const uint32_t head = kv_head * p.a.group + member / p.a.rows;
         if (node >= e.nodes) continue;
-        // (the row set began in range c0: its second partial unless it began exactly there)
+        // (the row set began in range c0, behind its first block or at it: the second partial; the
+        // others began with it)
         auto slot = [&](uint32_t c) {
-            const uint32_t which = range_begin(total, c, ctas) > first ? 0u : 1u;
-            return p.partial + (static_cast<uint64_t>(c) * 2 + which) * p.slot_floats;
+            return p.partial + (static_cast<uint64_t>(c) * 2 + (c == c0 ? 1u : 0u)) * p.slot_floats;
         };
         float top = __int_as_float(0xFF800000);
         for (uint32_t c = c0 + lane; c <= c1; c += 32) {
             const float* at = slot(c);
-            if (at[static_cast<uint64_t>(p.row_cap) * (width + 1) + r] != 0.0f) {
-                top = fmaxf(top, at[static_cast<uint64_t>(p.row_cap) * width + r]);
-            }
+            const float part = at[static_cast<uint64_t>(p.row_cap) * (width + 1) + r];
+            const float high = at[static_cast<uint64_t>(p.row_cap) * width + r];
+            if (part != 0.0f) top = fmaxf(top, high);
         }
         for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
         float sum = 0.0f, o[kMaxWidth / 32] = {};
         for (uint32_t base = c0; base <= c1; base += 32) {
-            // Every lane has one range's factor ready; all lanes then add it up in order.
+            // Every lane has one range's factor ready; all lanes then add the ranges up in order,
+            // eight reads ahead.
             float factor = 0.0f, part = 0.0f;
             if (base + lane <= c1) {
                 const float* at = slot(base + lane);
                 part = at[static_cast<uint64_t>(p.row_cap) * (width + 1) + r];
-                if (part != 0.0f) {
-                    factor = exp2_fast((at[static_cast<uint64_t>(p.row_cap) * width + r] - top) * p.scale_log2);
-                }
+                const float high = at[static_cast<uint64_t>(p.row_cap) * width + r];
+                if (part != 0.0f) factor = exp2_fast((high - top) * p.scale_log2);
             }
             const uint32_t count = min(32u, c1 - base + 1);
-            for (uint32_t i = 0; i < count; ++i) {
-                const float f = __shfl_sync(0xffffffffu, factor, i), l = __shfl_sync(0xffffffffu, part, i);
-                if (l == 0.0f) continue;        // nothing seen in that range
-                sum = __fmaf_rn(l, f, sum);
-                const float* at = slot(base + i) + static_cast<uint64_t>(r) * width;
+            constexpr uint32_t kAhead = 8;
+            for (uint32_t i0 = 0; i0 < count; i0 += kAhead) {
+                float v[kAhead][kMaxWidth / 32];
 #pragma unroll
-                for (uint32_t k = 0; k < kMaxWidth / 32; ++k) {
-                    if (lane + 32 * k < width) o[k] = __fmaf_rn(at[lane + 32 * k], f, o[k]);
+                for (uint32_t i = 0; i < kAhead; ++i) {
+                    const float* at = slot(base + min(i0 + i, count - 1)) + static_cast<uint64_t>(r) * width;
+#pragma unroll
+                    for (uint32_t k = 0; k < kMaxWidth / 32; ++k) {
+                        v[i][k] = lane + 32 * k < width ? at[lane + 32 * k] : 0.0f;
+                    }
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < kAhead; ++i) {
+                    const float f = __shfl_sync(0xffffffffu, factor, (i0 + i) & 31u);
+                    const float l = __shfl_sync(0xffffffffu, part, (i0 + i) & 31u);
+                    if (i0 + i >= count || l == 0.0f) continue;     // nothing seen in that range
+                    sum = __fmaf_rn(l, f, sum);
+#pragma unroll
+                    for (uint32_t k = 0; k < kMaxWidth / 32; ++k) o[k] = __fmaf_rn(v[i][k], f, o[k]);
                 }
             }
         }
@@ -1069,10 +1161,14 @@ TreeShape tree_shape(const AttnParams& a) {
     return t;
 }
 
-uint32_t shared_bytes(const AttnParams& a, bool alternate, uint32_t* stages) {
+// Dynamic shared memory: the queries (one tile where both hold the same rows; a second buffer where
+// it fits) and the ring of key and value blocks.
+uint32_t shared_bytes(const AttnParams& a, TcParams* p) {
     const uint32_t block = a.width * kTileRows * 2;
-    *stages = kRingBytes / block < kMaxStages ? kRingBytes / block : kMaxStages;
-    return 1024 + ((alternate ? 1u : 2u) + *stages) * block;
+    const uint32_t queries = (p->alternate ? 1u : 2u) * block;
+    p->stages = kRingBytes / block < kMaxStages ? kRingBytes / block : kMaxStages;
+    p->query_buffers = queries <= 32 * 1024 ? 2 : 1;
+    return 1024 + p->query_buffers * queries + p->stages * block;
 }
 
 }  // namespace
@@ -1130,7 +1226,7 @@ int launch_attention_tc(const AttnParams& a, bool tree, bool bf16, void* workspa
         p.row_cap = t.row_cap;
         p.slot_floats = t.slot_floats;
         p.partial = static_cast<float*>(workspace);
-        const uint32_t dynamic = shared_bytes(a, t.alternate != 0, &p.stages);
+        const uint32_t dynamic = shared_bytes(a, &p);
         return bf16 ? launch_leaf<LeafBf16, true>(p, t.ctas, dynamic, &t, stream)
                     : launch_leaf<LeafF16, true>(p, t.ctas, dynamic, &t, stream);
     }
@@ -1145,7 +1241,7 @@ int launch_attention_tc(const AttnParams& a, bool tree, bool bf16, void* workspa
     const uint64_t units = (static_cast<uint64_t>(a.rows) / (2 * p.tile_rows) + (a.batch < a.rows ? a.batch : a.rows))
             * p.head_tiles;
     if (units > 0x7FFFFFFFull) return fail(IOMB_ERR_UNSUPPORTED, "sdpa_packed: too many rows for one launch");
-    const uint32_t dynamic = shared_bytes(a, false, &p.stages);
+    const uint32_t dynamic = shared_bytes(a, &p);
     return bf16 ? launch_leaf<LeafBf16, false>(p, static_cast<uint32_t>(units), dynamic, nullptr, stream)
                 : launch_leaf<LeafF16, false>(p, static_cast<uint32_t>(units), dynamic, nullptr, stream);
 }
