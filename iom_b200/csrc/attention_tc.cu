@@ -3,14 +3,16 @@
 //
 // One CTA works on two tiles, A and B, of 128 score rows each. Per step of 64 tokens and tile
 //   S = Q K^T          tcgen05.mma, both operands in shared memory, S in tensor memory (FP32)
-//   P = exp2(c S - c m) softmax warpgroup of the tile: one thread per row, S read back from
-//                      tensor memory, P (16-bit) written over S
+//   P = exp2(c S - c m) softmax warps of the tile: S read back from tensor memory, P (16-bit)
+//                      written over it
 //   O += P V           tcgen05.mma, P from tensor memory, V from shared memory, O in tensor memory
-// with the running maximum m and sum l of each row in its thread. O is rescaled only when a
+// with the running maximum m and sum l of each row in its threads. O is rescaled only when a
 // row's maximum grows by more than 2^8 (P then stays below 2^8, far from any overflow); the sum
 // takes the unrounded exponentials. S has two buffers per tile: the scores of the next step are
-// there when the softmax of this one ends, so the exponentials, which bound the kernel (16 a
-// clock and SM), run without a pause.
+// on their way while the softmax of this one runs. The exponentials (16 a clock and SM) bound
+// the kernel at D = 64, the matrix instructions at D = 128; two threads share a row (32 tokens of
+// a step each, agreeing on the maximum), so that four warps per scheduler hide each other's
+// waits: with one thread per row and two warps a step took 1.5 times as long.
 //
 // The library's 16x16 tiles feed the matrix instructions without any re-layout: a tile row is 32
 // bytes, so a column of tiles is a K-major operand with 32-byte swizzle and K = 16 (one
@@ -31,10 +33,8 @@
 // but also garbage under the mask, which the matrix instruction multiplies by zero) is computed
 // again by attend_row, which reads visible tokens only.
 //
-// Warps: 0-3 softmax of A, 4-7 softmax of B, 8 issues the matrix instructions, 9 the copies, 10
-// and 11 bring the queries of a tree call's next row set while the last one is worked on. The
-// last four hand registers to the softmax (2 x 128 x 208 + 128 x 80 of the 384 x 168 a CTA
-// starts with).
+// Warps: 0-7 softmax of A, 8-15 softmax of B, 16 issues the matrix instructions, 17 the copies,
+// 18 and 19 bring the queries of a tree call's next row set while the last one is worked on.
 // Every wait is bounded; one that gives up ends all roles and is counted.
 #include <cuda.h>
 
@@ -45,8 +45,9 @@
 namespace iomb {
 namespace {
 
-constexpr uint32_t kThreads = 384;
-constexpr uint32_t kSoftmaxWarps = 8;
+constexpr uint32_t kThreads = 640;
+constexpr uint32_t kSoftmaxWarps = 16;
+constexpr uint32_t kProductWarp = 16, kCopyWarp = 17, kQueryWarp = 18, kQueryThreads = 64;
 constexpr uint32_t kTileRows = 128;
 constexpr uint32_t kMaxWidth = 128;
 constexpr uint32_t kMaxStages = 8;
@@ -113,13 +114,21 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatil
     *stop = 1;
     return false;
 }
-// Whether any of the 256 softmax threads says so; a barrier for them.
-__device__ __forceinline__ bool any_of_softmax(bool mine) {
+// Whether any of `threads` threads says so; a barrier for them. Ids: 1 all softmax threads, 2 to 9
+// the two warps of 32 rows, 10 the query warps.
+__device__ __forceinline__ bool any_of(uint32_t id, uint32_t threads, bool mine) {
     uint32_t any;
-    asm volatile("{\n\t.reg .pred mine, any;\n\tsetp.ne.u32 mine, %1, 0;\n\t"
-                 "barrier.cta.red.or.pred any, 1, 256, mine;\n\tselp.u32 %0, 1, 0, any;\n\t}"
-                 : "=r"(any) : "r"(mine ? 1u : 0u) : "memory");
+    asm volatile("{\n\t.reg .pred mine, any;\n\tsetp.ne.u32 mine, %3, 0;\n\t"
+                 "barrier.cta.red.or.pred any, %1, %2, mine;\n\tselp.u32 %0, 1, 0, any;\n\t}"
+                 : "=r"(any) : "r"(id), "r"(threads), "r"(mine ? 1u : 0u) : "memory");
     return any != 0;
+}
+__device__ __forceinline__ void copy16(uint32_t shared, const void* global) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared), "l"(global) : "memory");
+}
+__device__ __forceinline__ void copies_done() {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 // 128 tokens x D of one plane: tile rows [tile_row, tile_row + 8), every tile column.
 __device__ __forceinline__ void copy_block(uint32_t dst, const CUtensorMap* map, uint64_t* bar, uint32_t tile_row,
@@ -147,18 +156,6 @@ __device__ __forceinline__ void tmem_load32(uint32_t address, uint32_t* r) {
               "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
             : "r"(address));
 }
-__device__ __forceinline__ void tmem_store32(uint32_t address, const uint32_t* r) {
-    asm volatile(
-            "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-            "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-            "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
-            ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-              "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-              "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-              "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
-              "r"(address)
-            : "memory");
-}
 __device__ __forceinline__ void tmem_load16(uint32_t address, uint32_t* r) {
     asm volatile(
             "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -175,10 +172,6 @@ __device__ __forceinline__ void tmem_store16(uint32_t address, const uint32_t* r
               "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
               "r"(address)
             : "memory");
-}
-
-__device__ __forceinline__ void store_shared(uint32_t address, uint4 v) {
-    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(address), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
 // Shared-memory operand with 32-byte swizzle. Groups of eight 32-byte rows lie 256 bytes apart
@@ -436,13 +429,16 @@ __device__ __noinline__ void redo_row(const AttnParams& p, uint32_t b, uint32_t 
 struct Shared {
     uint64_t full[kMaxStages], empty[kMaxStages];
     uint64_t scores[2][2], weights[2][2];       // per tile and buffer: S written, P written
-    uint64_t values[2];                         // per tile: O holds one more step
+    uint64_t values[2], done[2];                // per tile: O holds one more step, the piece's last one
     uint64_t queries[2], queries_free[2];       // a piece's queries are there; its scores are computed
     uint64_t piece_free[2];                     // nobody reads the piece any more
     uint64_t drain;
     uint32_t tmem, stop, run;
     Piece pieces[2];
     Walk walk;                                  // tree
+    float high[2][2][2][kTileRows];             // per tile, buffer and half: a row's maximum
+    float part[2][2][kTileRows];                // per tile and half: a row's sum
+    uint32_t bad[2][2][4];                      // per tile, half and warp: rows to be computed again
     float other[2][kTileRows];                  // m and l of tile B (same rows)
     uint32_t mask[2][kMaxTreeNodes * kMaskWords];       // ancestors and the node itself
     int16_t parent[kMaxTreeNodes];
@@ -480,11 +476,13 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                 if (blockIdx.x == 0) *p.a.status = ok ? 0u : 1u;
             }
         }
-    } else if (warp == 8) {
+    } else if (warp == kProductWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(shared_address(&sh.tmem)), "r"(kTmemColumns) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-    } else if (warp == 9 && lane == 0) {
+    } else if (warp == kCopyWarp && lane == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&k_map)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&v_map)) : "memory");
         for (uint32_t s = 0; s < kMaxStages; ++s) {
             bar_init(&sh.full[s], 1);
             bar_init(&sh.empty[s], 1);
@@ -492,9 +490,10 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
         for (uint32_t x = 0; x < 2; ++x) {
             for (uint32_t i = 0; i < 2; ++i) {
                 bar_init(&sh.scores[x][i], 1);
-                bar_init(&sh.weights[x][i], 4);
+                bar_init(&sh.weights[x][i], kSoftmaxWarps / 2);
             }
             bar_init(&sh.values[x], 1);
+            bar_init(&sh.done[x], 1);
             bar_init(&sh.queries[x], TREE ? 2 : kSoftmaxWarps);
             bar_init(&sh.queries_free[x], 1);
             bar_init(&sh.piece_free[x], kSoftmaxWarps);
@@ -509,134 +508,139 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
     if constexpr (TREE) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem = sh.tmem;
     const bool run = sh.run != 0;
-    if (warp < kSoftmaxWarps) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    else asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
 
     if (run && warp < kSoftmaxWarps) {
-        // ---- softmax, one thread per row ------------------------------------------------------------
-        const uint32_t x = warp / 4, m = threadIdx.x & 127u;
+        // ---- softmax, two threads per row -------------------------------------------------------------
+        const uint32_t x = warp / 8, half = (warp / 4) & 1u, m = (warp & 3u) * 32 + lane;
         const uint32_t lanes = (warp & 3u) << 21;               // this warp's 32 tensor memory lanes
         const uint32_t s_at = tmem + lanes + x * 128, o_at = tmem + lanes + 256 + x * 128;
+        const uint32_t rows_id = 2 + x * 4 + (warp & 3u);       // the barrier of the rows' two warps
         const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
-        uint32_t steps_done = 0;                                // of this tile, over all pieces
+        const bool join = TREE && p.alternate;
+        // The head columns this thread scales and stores: its half, in tile columns.
+        const uint32_t c_begin = half == 0 ? 0 : (slices + 1) / 2, c_end = half == 0 ? (slices + 1) / 2 : slices;
+        uint32_t steps_done = 0, pieces_done = 0;               // of this tile, over all pieces
+        uint32_t head = 0, row = 0, member = m;                 // (the same in every piece while the tiles hold the same rows)
+        if (join) {
+            head = member / p.a.rows;
+            row = member % p.a.rows;
+        }
         bool alive = true;
         for (uint32_t turn = 0; ; ++turn) {
-            const uint32_t buffer = turn & 1u;
+            const uint32_t buffer = TREE ? turn & 1u : 0u;
             if constexpr (TREE) {
                 alive = __all_sync(0xffffffffu, bar_wait(&sh.queries[buffer], (turn / 2) & 1u, stop, kLongWaitCycles));
-                if (p.alternate) alive = !any_of_softmax(!alive);       // (one answer: barriers follow)
+                // (one answer for all whose barriers follow)
+                if (join) alive = !any_of(1, kSoftmaxWarps * 32, !alive);
+                else alive = !any_of(rows_id, 64, !alive);
                 if (!alive) break;
             }
-            const Piece& piece = sh.pieces[TREE ? buffer : 0];
+            const Piece& piece = sh.pieces[buffer];
             if (piece.blocks == 0) break;
             const uint32_t n = piece.steps[x], start = piece.start;
             // This thread's row.
-            uint32_t head, row;
+            uint32_t q_head;
             bool valid;
             if constexpr (TREE) {
-                const uint32_t member = (p.alternate ? 0u : piece.pair * 256 + x * 128) + m;
-                head = piece.kv_head * p.a.group + member / p.a.rows;
-                row = member % p.a.rows;
+                if (!join) {
+                    member = piece.pair * 256 + x * 128 + m;
+                    head = member / p.a.rows;
+                    row = member % p.a.rows;
+                }
+                q_head = piece.kv_head * p.a.group + head;
                 valid = member < p.members && row < piece.nodes;
             } else {
-                head = piece.pair * p.pack + m / p.tile_rows;
+                q_head = piece.pair * p.pack + m / p.tile_rows;
                 row = piece.row0 + x * p.tile_rows + m % p.tile_rows;
                 valid = row < piece.end;
             }
             const bool busy = __any_sync(0xffffffffu, valid) && n != 0;
             if constexpr (!TREE) {
-                // Q: 32 bytes of a tile row at a time, into the swizzled K-major operand.
-                if (n != 0) {
-                    const uint64_t plane = attn_plane(p.a.q, piece.b, head);
-                    const uint32_t dst = q_base + x * block_bytes + m * 32;
-                    const uint32_t flip = ((m >> 2) & 1u) * 16;
-                    for (uint32_t c = 0; c < slices; ++c) {
-                        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-                        if (valid) {
-                            const uint4* src = reinterpret_cast<const uint4*>(attn_piece(p.a.q, plane, row, c));
-                            lo = src[0];
-                            hi = src[1];
-                        }
-                        store_shared(dst + c * 4096 + flip, lo);
-                        store_shared(dst + c * 4096 + (16 - flip), hi);
+                // Q into the swizzled K-major operand, each half every other 32 bytes of a tile row. (What
+                // the rows that are not there hold reaches only results nobody stores.)
+                if (valid && n != 0) {
+                    const uint64_t plane = attn_plane(p.a.q, piece.b, q_head);
+                    const uint32_t dst = q_base + x * block_bytes + m * 32, flip = ((m >> 2) & 1u) * 16;
+                    for (uint32_t c = half; c < slices; c += 2) {
+                        const unsigned char* src = attn_piece(p.a.q, plane, row, c);
+                        copy16(dst + c * 4096 + flip, src);
+                        copy16(dst + c * 4096 + (16 - flip), src + 16);
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
+                copies_done();
                 __syncwarp();
                 if (lane == 0) bar_arrive(&sh.queries[0]);
             }
 
             const float kNone = __int_as_float(0xFF800000);
-            float top = kNone, sum = 0.0f;                      // running maximum (of S) and sum
-            const uint32_t first = piece.first_token + (TREE && p.alternate ? x * kStep : 0u);
-            const uint32_t stride = TREE && p.alternate ? kKvBlock : kStep;
+            float top = kNone, sum = 0.0f;                      // running maximum (of S) and this half's sum
+            const uint32_t first = piece.first_token + (join ? x * kStep : 0u) + half * 32;
+            const uint32_t stride = join ? kKvBlock : kStep;
             // Tokens from here on may be hidden from some row of the tile.
             const uint32_t clear = TREE ? start : piece.row0 + x * p.tile_rows + 1;
             for (uint32_t step = 0; step < n; ++step, ++steps_done) {
                 const uint32_t buf = steps_done & 1u, phase = (steps_done >> 1) & 1u;
-                // (one answer per warp)
-                alive = __all_sync(0xffffffffu, bar_wait(&sh.scores[x][buf], phase, stop));
-                if (!alive) break;
+                const bool there = bar_wait(&sh.scores[x][buf], phase, stop);
+                __syncwarp();
                 tmem_after_sync();
                 if (busy) {
-                    uint32_t s[kStep];
+                    uint32_t s[32];
                     const uint32_t at = s_at + buf * kStep;
-                    tmem_load32(at, s);
-                    tmem_load32(at + 32, s + 32);
+                    tmem_load32(at + half * 32, s);
                     const uint32_t token = first + step * stride;
-                    const bool masked = token + kStep > clear || (!TREE && token < start);
                     tmem_wait_load();
-                    if (masked) {
-                        uint32_t see[kStep / 32];
-#pragma unroll
-                        for (int w = 0; w < static_cast<int>(kStep / 32); ++w) {
-                            const int32_t from = static_cast<int32_t>(token) + 32 * w;
-                            if constexpr (!TREE) {
-                                see[w] = range_word(static_cast<int32_t>(start) - from, static_cast<int32_t>(row) - from);
-                            } else if (p.a.parents == nullptr) {
-                                see[w] = range_word(0, static_cast<int32_t>(start + row) - from);
-                            } else {
-                                see[w] = range_word(0, static_cast<int32_t>(start) - 1 - from);
-                                const int32_t rel = from - static_cast<int32_t>(start);
-                                if (valid && rel > -32 && rel < static_cast<int32_t>(kMaxTreeNodes)) {
-                                    const uint32_t* words = sh.mask[buffer] + row * kMaskWords;
-                                    if (rel < 0) {
-                                        see[w] |= words[0] << -rel;
-                                    } else {
-                                        const uint32_t i = rel / 32;
-                                        see[w] |= __funnelshift_r(words[i], i + 1 < kMaskWords ? words[i + 1] : 0u, rel % 32);
-                                    }
+                    if (token + 32 > clear || (!TREE && token < start)) {
+                        uint32_t see;
+                        const int32_t from = static_cast<int32_t>(token);
+                        if constexpr (!TREE) {
+                            see = range_word(static_cast<int32_t>(start) - from, static_cast<int32_t>(row) - from);
+                        } else if (p.a.parents == nullptr) {
+                            see = range_word(0, static_cast<int32_t>(start + row) - from);
+                        } else {
+                            see = range_word(0, static_cast<int32_t>(start) - 1 - from);
+                            const int32_t rel = from - static_cast<int32_t>(start);
+                            if (valid && rel > -32 && rel < static_cast<int32_t>(kMaxTreeNodes)) {
+                                const uint32_t* words = sh.mask[buffer] + row * kMaskWords;
+                                if (rel < 0) {
+                                    see |= words[0] << -rel;
+                                } else {
+                                    const uint32_t i = rel / 32;
+                                    see |= __funnelshift_r(words[i], i + 1 < kMaskWords ? words[i + 1] : 0u, rel % 32);
                                 }
                             }
-                            if (!valid) see[w] = 0;
                         }
+                        if (!valid) see = 0;
 #pragma unroll
-                        for (int c = 0; c < static_cast<int>(kStep); ++c) {
-                            if (!((see[c / 32] >> (c % 32)) & 1u)) s[c] = 0xFF800000u;
+                        for (int c = 0; c < 32; ++c) {
+                            if (!((see >> c) & 1u)) s[c] = 0xFF800000u;
                         }
                     }
                     float best[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) best[i] = fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 4]));
 #pragma unroll
-                    for (int c = 8; c < static_cast<int>(kStep); c += 8) {
+                    for (int c = 8; c < 32; c += 8) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             best[i] = fmaxf(fmaxf(best[i], __uint_as_float(s[c + i])), __uint_as_float(s[c + i + 4]));
                         }
                     }
-                    const float high = fmaxf(top, fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])));
+                    // The row's two threads agree on its maximum (and on whether to go on).
+                    float high = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
+                    sh.high[x][buf][half][m] = high;
+                    if (any_of(rows_id, 64, !there || !alive)) { alive = false; break; }
+                    high = fmaxf(top, fmaxf(high, sh.high[x][buf][half ^ 1u][m]));
                     // The first tokens seen, or a maximum that grew beyond what P may: a new reference.
                     const bool fresh = top == kNone;
                     const bool grow = !fresh && (high - top) * p.scale_log2 > kRescale;
                     if (__any_sync(0xffffffffu, grow)) {
                         // (not the first step: O holds the steps before this one once they are done)
-                        alive = __all_sync(0xffffffffu, bar_wait(&sh.values[x], (steps_done - 1) & 1u, stop));
-                        if (!alive) break;
+                        if (!bar_wait(&sh.values[x], (steps_done - 1) & 1u, stop)) alive = false;
+                        alive = __all_sync(0xffffffffu, alive);     // (acted upon where both warps meet next)
                         tmem_after_sync();
                         const float factor = grow ? exp2_fast((top - high) * p.scale_log2) : 1.0f;
                         sum *= factor;
-                        for (uint32_t c = 0; c < slices; ++c) {
+                        for (uint32_t c = c_begin; c < c_end; ++c) {
                             uint32_t o[16];
                             tmem_load16(o_at + c * 16, o);
                             tmem_wait_load();
@@ -648,44 +652,50 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                     if (fresh || grow) top = high;
                     const float shift = top == kNone ? 0.0f : -(top * p.scale_log2);
                     const uint64_t shift2 = pair(shift, shift);
-                    uint64_t sums[4] = {0, 0, 0, 0};
+                    uint64_t sums[2] = {0, 0};
 #pragma unroll
-                    for (int c = 0; c < static_cast<int>(kStep); c += 2) {
+                    for (int c = 0; c < 32; c += 2) {
                         float e0, e1;
                         unpair(fma2(pair(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), scale2, shift2), e0, e1);
                         e0 = exp2_fast(e0);
                         e1 = exp2_fast(e1);
-                        sums[(c / 2) % 4] = add2(sums[(c / 2) % 4], pair(e0, e1));
+                        sums[(c / 2) % 2] = add2(sums[(c / 2) % 2], pair(e0, e1));
                         s[c / 2] = Leaf::pack(e0, e1);
                     }
-                    tmem_store32(at, s);
+                    tmem_store16(at + half * 16, s);
                     float a, b;
-                    unpair(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])), a, b);
+                    unpair(add2(sums[0], sums[1]), a, b);
                     sum += a + b;
                     tmem_wait_store();
+                } else if (!__all_sync(0xffffffffu, there)) {
+                    alive = false;
+                    break;
                 }
                 tmem_before_sync();
                 __syncwarp();
                 if (lane == 0) bar_arrive(&sh.weights[x][buf]);
             }
             if (alive && n != 0) {
-                // The last two steps, one after the other: a wait tells a phase from the one before
-                // it only, and the scores of the last step say no more than that the step three
-                // back is done.
-                if (n > 1) alive = bar_wait(&sh.values[x], (steps_done - 2) & 1u, stop);
-                alive = __all_sync(0xffffffffu, alive && bar_wait(&sh.values[x], (steps_done - 1) & 1u, stop));
+                // (a barrier of its own: when a warp comes here none, one or both of the last two steps
+                // may be done, and a parity does not tell the first case from the last)
+                alive = __all_sync(0xffffffffu, bar_wait(&sh.done[x], pieces_done & 1u, stop));
+                ++pieces_done;
                 tmem_after_sync();
             }
             // ---- results ---------------------------------------------------------------------------
-            const bool join = TREE && p.alternate;
+            if (busy) {
+                sh.part[x][half][m] = sum;
+                alive = !any_of(rows_id, 64, !alive);
+                sum += sh.part[x][half ^ 1u][m];
+            }
             const bool second = join && piece.steps[1] != 0;        // tile B holds part of the sum
             float mine = 1.0f, its = 0.0f;                          // factors of the two tiles' O
             if (join) {
-                if (x == 1) {
+                if (x == 1 && half == 0) {
                     sh.other[0][m] = top;
                     sh.other[1][m] = sum;
                 }
-                asm volatile("bar.sync 1, 256;" ::: "memory");
+                alive = !any_of(1, kSoftmaxWarps * 32, !alive);
                 if (x == 0 && second) {
                     const float top_b = sh.other[0][m], sum_b = sh.other[1][m];
                     const float high = fmaxf(top, top_b);
@@ -700,73 +710,69 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                 const float inverse = whole ? 1.0f / sum : 1.0f;
                 bool bad = !(sum > 0.0f && sum <= 3.0e38f);
                 const uint64_t plane = attn_plane(p.a.out, piece.b, 0);
-                const uint32_t column = head * slices, local = (TREE && !p.alternate ? x * 128 : 0u) + m;
+                const uint32_t column = q_head * slices, local = (TREE && !p.alternate ? x * 128 : 0u) + m;
                 float* const slot = p.partial + static_cast<uint64_t>(blockIdx.x * 2 + piece.slot) * p.slot_floats;
-                for (uint32_t c = 0; c < slices; c += 2) {
-                    // (32 columns at a time; those behind the head's width are not used)
-                    uint32_t o[32], o2[32];
-                    tmem_load32(o_at + c * 16, o);
-                    if (second) tmem_load32(o_at + 128 + c * 16, o2);
+                for (uint32_t c = c_begin; c < c_end; ++c) {
+                    uint32_t o[16], o2[16];
+                    tmem_load16(o_at + c * 16, o);
+                    if (second) tmem_load16(o_at + 128 + c * 16, o2);
                     tmem_wait_load();
                     if (second) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
+                        for (int i = 0; i < 16; ++i) {
                             float v = mine == 0.0f ? 0.0f : __uint_as_float(o[i]) * mine;
                             if (its != 0.0f) v = __fmaf_rn(__uint_as_float(o2[i]), its, v);
                             o[i] = __float_as_uint(v);
                         }
                     }
+                    if (whole) {
+                        uint32_t packed[8];
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        if (c + half >= slices) break;
-                        uint32_t* const part = o + 16 * half;
-                        if (whole) {
-                            uint32_t packed[8];
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const float lo = __uint_as_float(part[2 * i]) * inverse, hi = __uint_as_float(part[2 * i + 1]) * inverse;
-                                bad = bad || !(fabsf(lo) <= 3.4028234e38f) || !(fabsf(hi) <= 3.4028234e38f);
-                                packed[i] = canonical_pair<Leaf>(Leaf::pack(lo, hi));
-                            }
-                            if (valid) {
-                                store_u8_stream(attn_out_piece(p.a.out, plane, row, column + c + half),
-                                                make_uint4(packed[0], packed[1], packed[2], packed[3]),
-                                                make_uint4(packed[4], packed[5], packed[6], packed[7]));
-                            }
-                        } else if (valid) {
-                            uint4* to = reinterpret_cast<uint4*>(slot + static_cast<uint64_t>(local) * width + (c + half) * 16);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                to[i] = make_uint4(part[4 * i], part[4 * i + 1], part[4 * i + 2], part[4 * i + 3]);
-                            }
+                        for (int i = 0; i < 8; ++i) {
+                            const float lo = __uint_as_float(o[2 * i]) * inverse, hi = __uint_as_float(o[2 * i + 1]) * inverse;
+                            bad = bad || !(fabsf(lo) <= 3.4028234e38f) || !(fabsf(hi) <= 3.4028234e38f);
+                            packed[i] = canonical_pair<Leaf>(Leaf::pack(lo, hi));
                         }
+                        if (valid) {
+                            store_u8_stream(attn_out_piece(p.a.out, plane, row, column + c),
+                                            make_uint4(packed[0], packed[1], packed[2], packed[3]),
+                                            make_uint4(packed[4], packed[5], packed[6], packed[7]));
+                        }
+                    } else if (valid) {
+                        uint4* to = reinterpret_cast<uint4*>(slot + static_cast<uint64_t>(local) * width + c * 16);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) to[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     }
                 }
                 if (whole) {
+                    // Rows with a result that is not finite, in either half: once more, behind both
+                    // halves' stores.
                     uint32_t again = __ballot_sync(0xffffffffu, bad && valid);
-                    while (again != 0) {
-                        const int who = __ffs(again) - 1;
-                        again &= again - 1;
-                        __syncwarp();
-                        redo_row<Leaf, TREE>(p.a, piece.b, __shfl_sync(0xffffffffu, head, who),
-                                             __shfl_sync(0xffffffffu, row, who), start);
+                    if (lane == 0) sh.bad[x][half][warp & 3u] = again;
+                    any_of(rows_id, 64, false);
+                    again |= sh.bad[x][half ^ 1u][warp & 3u];
+                    if (half == 0) {
+                        while (again != 0) {
+                            const int who = __ffs(again) - 1;
+                            again &= again - 1;
+                            redo_row<Leaf, TREE>(p.a, piece.b, __shfl_sync(0xffffffffu, q_head, who),
+                                                 __shfl_sync(0xffffffffu, row, who), start);
+                        }
                     }
-                } else if (valid) {
+                } else if (valid && half == 0) {
                     slot[static_cast<uint64_t>(p.row_cap) * width + local] = top;
                     slot[static_cast<uint64_t>(p.row_cap) * (width + 1) + local] = sum;
                 }
             }
             if constexpr (!TREE) break;
             tmem_before_sync();
-            if (join) {
-                // Both tiles' results are out of tensor memory; one give-up ends both.
-                alive = !any_of_softmax(!alive || *stop != 0);
-            }
+            // Both tiles' results are out of tensor memory; one give-up ends both.
+            if (join) alive = !any_of(1, kSoftmaxWarps * 32, !alive || *stop != 0);
             if (!alive) break;
             __syncwarp();
             if (lane == 0) bar_arrive(&sh.piece_free[buffer]);
         }
-    } else if (run && warp == 8) {
+    } else if (run && warp == kProductWarp) {
         // ---- matrix instructions ---------------------------------------------------------------------
         const uint32_t leader = elect_lane();
         const uint32_t kind_s = product_descriptor(Leaf::kFormat, kStep, false);
@@ -840,6 +846,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                                    v + t * (512 >> 4), kind_o, j + t);
                     }
                     mma_commit(leader, &sh.values[x]);
+                    if (j + 1 == steps) mma_commit(leader, &sh.done[x]);
                     if (next < steps) {
                         // (the keys two steps on come behind these values: the order of the copies)
                         if (k_have <= next_block) take(k_have, k_slot);
@@ -860,7 +867,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             while (!bar_test(&sh.drain, 0) && clock64() - start < kWaitCycles) {}
         }
         __syncwarp();
-    } else if (run && warp == 9) {
+    } else if (run && warp == kCopyWarp) {
         // ---- copies, one thread -----------------------------------------------------------------------------
         if (lane == 0) {
             uint32_t issued = 0;
@@ -908,7 +915,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
     } else if (TREE && run) {
         // ---- queries, pieces and ancestor masks, two warps -----------------------------------------------
         if constexpr (TREE) {
-            const uint32_t me = threadIdx.x - 10 * 32;
+            const uint32_t me = threadIdx.x - kQueryWarp * 32;
             Walk walk = sh.walk;
             Piece piece;
             bool alive = true;
@@ -921,22 +928,17 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                 const uint32_t place = p.query_buffers == 2 ? buffer : 0u;
                 const uint32_t used = p.query_buffers == 2 ? turn / 2 : turn;      // times the place was filled
                 if (go && used > 0) alive = alive && bar_wait(&sh.queries_free[place], (used - 1) & 1u, stop, kLongWaitCycles);
-                // (both warps go on or both give up)
-                uint32_t over;
-                asm volatile("{\n\t.reg .pred mine, any;\n\tsetp.ne.u32 mine, %1, 0;\n\t"
-                             "barrier.cta.red.or.pred any, 2, 64, mine;\n\tselp.u32 %0, 1, 0, any;\n\t}"
-                             : "=r"(over) : "r"(alive ? 0u : 1u) : "memory");
-                alive = over == 0;
+                alive = !any_of(10, kQueryThreads, !alive);     // (both warps go on or both give up)
                 if (!alive) break;
                 if (me == 0) sh.pieces[buffer] = piece;
                 if (go) {
                     if (p.a.parents != nullptr && piece.first_token + piece.blocks * kKvBlock > piece.start) {
                         const int32_t* parents = p.a.parents + static_cast<uint64_t>(piece.b) * p.a.rows;
-                        for (uint32_t i = me; i < piece.nodes; i += 64) {
+                        for (uint32_t i = me; i < piece.nodes; i += kQueryThreads) {
                             sh.parent[i] = static_cast<int16_t>(max(-1, tree_parent(parents, static_cast<int32_t>(i))));
                         }
-                        asm volatile("bar.sync 2, 64;" ::: "memory");
-                        for (uint32_t i = me; i < piece.nodes; i += 64) {
+                        asm volatile("bar.sync 10, 64;" ::: "memory");
+                        for (uint32_t i = me; i < piece.nodes; i += kQueryThreads) {
                             uint32_t* words = sh.mask[buffer] + i * kMaskWords;
                             for (uint32_t w = 0; w < kMaskWords; ++w) words[w] = 0;
                             for (int32_t at = static_cast<int32_t>(i); at >= 0; at = sh.parent[at]) {
@@ -949,22 +951,18 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                     const uint32_t offset = piece.pair * 256;
                     const uint32_t rows = min(p.alternate ? kTileRows : 2 * kTileRows, p.members - offset);
                     const uint32_t base = q_base + place * query_bytes;
-                    for (uint32_t c = 0; c < slices; ++c) {
-                        for (uint32_t r = me; r < rows; r += 64) {
-                            const uint32_t member = offset + r;
-                            const uint32_t head = piece.kv_head * p.a.group + member / p.a.rows;
-                            const uint4* src = reinterpret_cast<const uint4*>(
-                                    attn_piece(p.a.q, attn_plane(p.a.q, piece.b, head), member % p.a.rows, c));
-                            const uint4 lo = src[0], hi = src[1];
-                            const uint32_t m = r % kTileRows, flip = ((m >> 2) & 1u) * 16;
-                            const uint32_t to = base + (r / kTileRows) * block_bytes + c * 4096 + m * 32;
-                            store_shared(to + flip, lo);
-                            store_shared(to + (16 - flip), hi);
-                        }
+                    for (uint32_t r = me; r < rows * slices; r += kQueryThreads) {
+                        const uint32_t c = r / rows, local = r % rows, of_head = offset + local;
+                        const uint32_t q_head = piece.kv_head * p.a.group + of_head / p.a.rows;
+                        const unsigned char* src = attn_piece(p.a.q, attn_plane(p.a.q, piece.b, q_head), of_head % p.a.rows, c);
+                        const uint32_t m = local % kTileRows, flip = ((m >> 2) & 1u) * 16;
+                        const uint32_t to = base + (local / kTileRows) * block_bytes + c * 4096 + m * 32;
+                        copy16(to + flip, src);
+                        copy16(to + (16 - flip), src + 16);
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    copies_done();
                 }
-                asm volatile("bar.sync 2, 64;" ::: "memory");
+                asm volatile("bar.sync 10, 64;" ::: "memory");
                 if (lane == 0) bar_arrive(&sh.queries[buffer]);
                 if (!go) break;
             }
@@ -972,12 +970,12 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
     }
     if constexpr (TREE) {
         // (behind the copies, beside the last products)
-        if (warp == 9 && blockIdx.x == 0) warp_report_tree(p.a);
+        if (warp == kCopyWarp && blockIdx.x == 0) warp_report_tree(p.a);
     }
     tmem_before_sync();
     __syncthreads();
     tmem_after_sync();
-    if (warp == 8) {
+    if (warp == kProductWarp) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns));
         if (lane == 0 && sh.stop != 0) atomicAdd(&g_attention_timeouts, 1u);
     }
@@ -985,7 +983,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
 
 // Joins the partial sums of row sets whose blocks lie in several ranges: a warp per row, the
 // ranges in order. Reads a few KB per row; bound by the latency of two dependent reads.
-constexpr uint32_t kJoinRows = 32, kJoinWarps = 4;
+constexpr uint32_t kJoinWarps = 4, kJoinRows = kJoinWarps;     // rows per CTA: one per warp
 
 template <class Leaf>
 __global__ void __launch_bounds__(kJoinWarps * 32)
