@@ -1,18 +1,16 @@
 // Attention on the tensor cores: the kernel behind iomb_sdpa_packed and iomb_sdpa_tree for head
 // widths that are multiples of 16 up to 128.
 //
-// One CTA works on two tiles, A and B, of 128 score rows each. Per step of 64 tokens and tile
+// One CTA works on two tiles, A and B, of 128 score rows each. Per block of 128 tokens and tile
 //   S = Q K^T          tcgen05.mma, both operands in shared memory, S in tensor memory (FP32)
-//   P = exp2(c S - c m) softmax warps of the tile: S read back from tensor memory, P (16-bit)
-//                      written over it
+//   P = exp2(c S - c m) softmax warpgroup of the tile: one thread per row, S read back from
+//                      tensor memory, P (16-bit) written over S
 //   O += P V           tcgen05.mma, P from tensor memory, V from shared memory, O in tensor memory
-// with the running maximum m and sum l of each row in its threads. O is rescaled only when a
+// with the running maximum m and sum l of each row in its thread. O is rescaled only when a
 // row's maximum grows by more than 2^8 (P then stays below 2^8, far from any overflow); the sum
-// takes the unrounded exponentials. S has two buffers per tile: the scores of the next step are
-// on their way while the softmax of this one runs. The exponentials (16 a clock and SM) bound
-// the kernel at D = 64, the matrix instructions at D = 128; two threads share a row (32 tokens of
-// a step each, agreeing on the maximum), so that four warps per scheduler hide each other's
-// waits: with one thread per row and two warps a step took 1.5 times as long.
+// takes the unrounded exponentials. While one tile's softmax runs, the other tile's products do.
+// P is handed over in two halves, so that its product with V begins while the second half's
+// exponentials are still computed.
 //
 // The library's 16x16 tiles feed the matrix instructions without any re-layout: a tile row is 32
 // bytes, so a column of tiles is a K-major operand with 32-byte swizzle and K = 16 (one
@@ -23,8 +21,8 @@
 //   packed   `pack` heads of one key/value head x 128/pack consecutive rows, so that short
 //            sequences share a tile between heads; A and B are neighbouring row blocks
 //   tree     the (head, node) pairs of one key/value head. Up to 128 pairs: both tiles hold the
-//            same rows, A takes the first half of every block of 128 tokens and B the second,
-//            joined at the end. More: A and B hold 128 pairs each and share the tokens
+//            same rows and take alternate token blocks, joined at the end. More: A and B hold
+//            128 pairs each and share the token blocks
 // The tree call cuts the token blocks of all sequences and heads into equal ranges, one per CTA.
 // A row whose blocks lie in several ranges leaves partial (m, l, O) in the workspace and a second
 // kernel joins them, in the order of the ranges.
@@ -33,8 +31,10 @@
 // but also garbage under the mask, which the matrix instruction multiplies by zero) is computed
 // again by attend_row, which reads visible tokens only.
 //
-// Warps: 0-7 softmax of A, 8-15 softmax of B, 16 issues the matrix instructions, 17 the copies,
-// 18 and 19 bring the queries of a tree call's next row set while the last one is worked on.
+// Warps: 0-3 softmax of A, 4-7 softmax of B, 8 issues the matrix instructions, 9 the copies, 10
+// and 11 bring the queries of a tree call's next row set while the last one is worked on. The
+// last four hand registers to the softmax (2 x 128 x 208 + 128 x 80 of the 384 x 168 a CTA
+// starts with).
 // Every wait is bounded; one that gives up ends all roles and is counted.
 #include <cuda.h>
 
@@ -45,15 +45,14 @@
 namespace iomb {
 namespace {
 
-constexpr uint32_t kThreads = 640;
-constexpr uint32_t kSoftmaxWarps = 16;
-constexpr uint32_t kProductWarp = 16, kCopyWarp = 17, kQueryWarp = 18, kQueryThreads = 64;
+constexpr uint32_t kThreads = 384;
+constexpr uint32_t kSoftmaxWarps = 8;
+constexpr uint32_t kProductWarp = 8, kCopyWarp = 9, kQueryWarp = 10, kQueryThreads = 64;
 constexpr uint32_t kTileRows = 128;
 constexpr uint32_t kMaxWidth = 128;
 constexpr uint32_t kMaxStages = 8;
 constexpr uint32_t kRingBytes = 128 * 1024;
-constexpr uint32_t kStep = 64;                  // tokens per softmax step
-constexpr uint32_t kTmemColumns = 512;          // S of A and B: 2 x 64 at 0, 128; O of A and B: 256, 384
+constexpr uint32_t kTmemColumns = 512;          // S of A and B: 0, 128; O of A and B: 256, 384
 constexpr uint32_t kMaskWords = kMaxTreeNodes / 32;
 constexpr float kRescale = 8.0f;                // in powers of two
 // Bounds of the waits: about a second, and a quarter of a minute where the other side may be
@@ -114,13 +113,14 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatil
     *stop = 1;
     return false;
 }
-// Whether any of `threads` threads says so; a barrier for them. Ids: 1 all softmax threads, 2 to 9
-// the two warps of 32 rows, 10 the query warps.
-__device__ __forceinline__ bool any_of(uint32_t id, uint32_t threads, bool mine) {
+// Whether any of `threads` threads says so; a barrier for them. Ids: 1 all softmax threads, 2 the
+// query warps.
+template <uint32_t id, uint32_t threads>
+__device__ __forceinline__ bool any_of(bool mine) {
     uint32_t any;
     asm volatile("{\n\t.reg .pred mine, any;\n\tsetp.ne.u32 mine, %3, 0;\n\t"
                  "barrier.cta.red.or.pred any, %1, %2, mine;\n\tselp.u32 %0, 1, 0, any;\n\t}"
-                 : "=r"(any) : "r"(id), "r"(threads), "r"(mine ? 1u : 0u) : "memory");
+                 : "=r"(any) : "n"(id), "n"(threads), "r"(mine ? 1u : 0u) : "memory");
     return any != 0;
 }
 __device__ __forceinline__ void copy16(uint32_t shared, const void* global) {
@@ -155,6 +155,18 @@ __device__ __forceinline__ void tmem_load32(uint32_t address, uint32_t* r) {
               "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
               "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
             : "r"(address));
+}
+__device__ __forceinline__ void tmem_store32(uint32_t address, const uint32_t* r) {
+    asm volatile(
+            "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+            "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+            "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+            ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+              "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+              "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+              "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
+              "r"(address)
+            : "memory");
 }
 __device__ __forceinline__ void tmem_load16(uint32_t address, uint32_t* r) {
     asm volatile(
@@ -243,7 +255,7 @@ struct Piece {
     uint32_t b, kv_head, pair;  // sequence, key/value head, tile pair
     uint32_t first_token;       // multiple of 16: the first block's first row of k and v
     uint32_t blocks;            // blocks of 128 tokens; none: there are no more pieces
-    uint32_t steps[2];          // per tile, of 64 tokens
+    uint32_t steps[2];          // blocks per tile
     uint32_t end;               // rows of the sequence end here (packed), live rows (tree)
     uint32_t row0;              // packed: first row of tile A
     uint32_t start;             // packed: first row of the sequence; tree: rows before the tree
@@ -279,13 +291,8 @@ __device__ __forceinline__ bool next_piece(const TcParams& p, Walk& w, Piece& ou
     out.first_token = w.block * kKvBlock;
     out.blocks = take;
     out.end = e.length + e.nodes;
-    const uint32_t tokens = min(out.end - out.first_token, take * kKvBlock);
-    if (p.alternate) {
-        out.steps[0] = take;
-        out.steps[1] = tokens - (take - 1) * kKvBlock > kStep ? take : take - 1;
-    } else {
-        out.steps[0] = out.steps[1] = (tokens + kStep - 1) / kStep;
-    }
+    out.steps[0] = p.alternate ? (take + 1) / 2 : take;
+    out.steps[1] = p.alternate ? take / 2 : take;
     out.row0 = 0;
     out.start = e.length;
     out.nodes = e.nodes;
@@ -399,9 +406,9 @@ __device__ __forceinline__ bool plan_packed(const TcParams& p, uint32_t unit, Pi
     for (uint32_t x = 0; x < 2; ++x) {
         const uint32_t row = out.row0 + x * p.tile_rows;
         const uint32_t last = min(out.end, row + p.tile_rows);      // one behind the tile's last row
-        out.steps[x] = row < out.end ? (last - out.first_token + kStep - 1) / kStep : 0;
+        out.steps[x] = row < out.end ? (last - out.first_token + kKvBlock - 1) / kKvBlock : 0;
     }
-    out.blocks = (max(out.steps[0], out.steps[1]) + 1) / 2;
+    out.blocks = max(out.steps[0], out.steps[1]);
     out.nodes = 0;
     out.whole = 1;
     out.slot = 0;
@@ -428,17 +435,13 @@ __device__ __noinline__ void redo_row(const AttnParams& p, uint32_t b, uint32_t 
 
 struct Shared {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t scores[2][2], weights[2][2];       // per tile and buffer: S written, P written
-    uint64_t values[2], done[2];                // per tile: O holds one more step, the piece's last one
+    uint64_t scores[2], weights[2][2], done[2]; // per tile: S written, P written (halves), O complete
     uint64_t queries[2], queries_free[2];       // a piece's queries are there; its scores are computed
     uint64_t piece_free[2];                     // nobody reads the piece any more
     uint64_t drain;
     uint32_t tmem, stop, run;
     Piece pieces[2];
     Walk walk;                                  // tree
-    float high[2][2][2][kTileRows];             // per tile, buffer and half: a row's maximum
-    float part[2][2][kTileRows];                // per tile and half: a row's sum
-    uint32_t bad[2][2][4];                      // per tile, half and warp: rows to be computed again
     float other[2][kTileRows];                  // m and l of tile B (same rows)
     uint32_t mask[2][kMaxTreeNodes * kMaskWords];       // ancestors and the node itself
     int16_t parent[kMaxTreeNodes];
@@ -488,11 +491,9 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             bar_init(&sh.empty[s], 1);
         }
         for (uint32_t x = 0; x < 2; ++x) {
-            for (uint32_t i = 0; i < 2; ++i) {
-                bar_init(&sh.scores[x][i], 1);
-                bar_init(&sh.weights[x][i], kSoftmaxWarps / 2);
-            }
-            bar_init(&sh.values[x], 1);
+            bar_init(&sh.scores[x], 1);
+            bar_init(&sh.weights[x][0], kSoftmaxWarps / 2);
+            bar_init(&sh.weights[x][1], kSoftmaxWarps / 2);
             bar_init(&sh.done[x], 1);
             bar_init(&sh.queries[x], TREE ? 2 : kSoftmaxWarps);
             bar_init(&sh.queries_free[x], 1);
@@ -508,17 +509,16 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
     if constexpr (TREE) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem = sh.tmem;
     const bool run = sh.run != 0;
+    if (warp < kSoftmaxWarps) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
 
     if (run && warp < kSoftmaxWarps) {
-        // ---- softmax, two threads per row -------------------------------------------------------------
-        const uint32_t x = warp / 8, half = (warp / 4) & 1u, m = (warp & 3u) * 32 + lane;
+        // ---- softmax, one thread per row ---------------------------------------------------------------
+        const uint32_t x = warp / 4, m = (warp & 3u) * 32 + lane;
         const uint32_t lanes = (warp & 3u) << 21;               // this warp's 32 tensor memory lanes
         const uint32_t s_at = tmem + lanes + x * 128, o_at = tmem + lanes + 256 + x * 128;
-        const uint32_t rows_id = 2 + x * 4 + (warp & 3u);       // the barrier of the rows' two warps
         const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
         const bool join = TREE && p.alternate;
-        // The head columns this thread scales and stores: its half, in tile columns.
-        const uint32_t c_begin = half == 0 ? 0 : (slices + 1) / 2, c_end = half == 0 ? (slices + 1) / 2 : slices;
         uint32_t steps_done = 0, pieces_done = 0;               // of this tile, over all pieces
         uint32_t head = 0, row = 0, member = m;                 // (the same in every piece while the tiles hold the same rows)
         if (join) {
@@ -531,8 +531,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             if constexpr (TREE) {
                 alive = __all_sync(0xffffffffu, bar_wait(&sh.queries[buffer], (turn / 2) & 1u, stop, kLongWaitCycles));
                 // (one answer for all whose barriers follow)
-                if (join) alive = !any_of(1, kSoftmaxWarps * 32, !alive);
-                else alive = !any_of(rows_id, 64, !alive);
+                if (join) alive = !any_of<1, kSoftmaxWarps * 32>(!alive);
                 if (!alive) break;
             }
             const Piece& piece = sh.pieces[buffer];
@@ -556,12 +555,12 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             }
             const bool busy = __any_sync(0xffffffffu, valid) && n != 0;
             if constexpr (!TREE) {
-                // Q into the swizzled K-major operand, each half every other 32 bytes of a tile row. (What
-                // the rows that are not there hold reaches only results nobody stores.)
+                // Q, 32 bytes of a tile row at a time, into the swizzled K-major operand. (What the rows
+                // that are not there hold reaches only results nobody stores.)
                 if (valid && n != 0) {
                     const uint64_t plane = attn_plane(p.a.q, piece.b, q_head);
                     const uint32_t dst = q_base + x * block_bytes + m * 32, flip = ((m >> 2) & 1u) * 16;
-                    for (uint32_t c = half; c < slices; c += 2) {
+                    for (uint32_t c = 0; c < slices; ++c) {
                         const unsigned char* src = attn_piece(p.a.q, plane, row, c);
                         copy16(dst + c * 4096 + flip, src);
                         copy16(dst + c * 4096 + (16 - flip), src + 16);
@@ -573,74 +572,70 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             }
 
             const float kNone = __int_as_float(0xFF800000);
-            float top = kNone, sum = 0.0f;                      // running maximum (of S) and this half's sum
-            const uint32_t first = piece.first_token + (join ? x * kStep : 0u) + half * 32;
-            const uint32_t stride = join ? kKvBlock : kStep;
+            float top = kNone, sum = 0.0f;                      // running maximum (of S) and sum
+            const uint32_t first = piece.first_token + (join ? x * kKvBlock : 0u);
+            const uint32_t stride = join ? 2 * kKvBlock : kKvBlock;
             // Tokens from here on may be hidden from some row of the tile.
             const uint32_t clear = TREE ? start : piece.row0 + x * p.tile_rows + 1;
             for (uint32_t step = 0; step < n; ++step, ++steps_done) {
-                const uint32_t buf = steps_done & 1u, phase = (steps_done >> 1) & 1u;
-                const bool there = bar_wait(&sh.scores[x][buf], phase, stop);
-                __syncwarp();
+                // (one answer per warp)
+                alive = __all_sync(0xffffffffu, bar_wait(&sh.scores[x], steps_done & 1u, stop));
+                if (!alive) break;
                 tmem_after_sync();
                 if (busy) {
-                    uint32_t s[32];
-                    const uint32_t at = s_at + buf * kStep;
-                    tmem_load32(at + half * 32, s);
+                    uint32_t s[kKvBlock];
+#pragma unroll
+                    for (int c = 0; c < static_cast<int>(kKvBlock); c += 32) tmem_load32(s_at + c, s + c);
                     const uint32_t token = first + step * stride;
                     tmem_wait_load();
-                    if (token + 32 > clear || (!TREE && token < start)) {
-                        uint32_t see;
-                        const int32_t from = static_cast<int32_t>(token);
-                        if constexpr (!TREE) {
-                            see = range_word(static_cast<int32_t>(start) - from, static_cast<int32_t>(row) - from);
-                        } else if (p.a.parents == nullptr) {
-                            see = range_word(0, static_cast<int32_t>(start + row) - from);
-                        } else {
-                            see = range_word(0, static_cast<int32_t>(start) - 1 - from);
-                            const int32_t rel = from - static_cast<int32_t>(start);
-                            if (valid && rel > -32 && rel < static_cast<int32_t>(kMaxTreeNodes)) {
-                                const uint32_t* words = sh.mask[buffer] + row * kMaskWords;
-                                if (rel < 0) {
-                                    see |= words[0] << -rel;
-                                } else {
-                                    const uint32_t i = rel / 32;
-                                    see |= __funnelshift_r(words[i], i + 1 < kMaskWords ? words[i + 1] : 0u, rel % 32);
+                    if (token + kKvBlock > clear || (!TREE && token < start)) {
+                        uint32_t see[kKvBlock / 32];
+#pragma unroll
+                        for (int w = 0; w < static_cast<int>(kKvBlock / 32); ++w) {
+                            const int32_t from = static_cast<int32_t>(token) + 32 * w;
+                            if constexpr (!TREE) {
+                                see[w] = range_word(static_cast<int32_t>(start) - from, static_cast<int32_t>(row) - from);
+                            } else if (p.a.parents == nullptr) {
+                                see[w] = range_word(0, static_cast<int32_t>(start + row) - from);
+                            } else {
+                                see[w] = range_word(0, static_cast<int32_t>(start) - 1 - from);
+                                const int32_t rel = from - static_cast<int32_t>(start);
+                                if (valid && rel > -32 && rel < static_cast<int32_t>(kMaxTreeNodes)) {
+                                    const uint32_t* words = sh.mask[buffer] + row * kMaskWords;
+                                    if (rel < 0) {
+                                        see[w] |= words[0] << -rel;
+                                    } else {
+                                        const uint32_t i = rel / 32;
+                                        see[w] |= __funnelshift_r(words[i], i + 1 < kMaskWords ? words[i + 1] : 0u, rel % 32);
+                                    }
                                 }
                             }
+                            if (!valid) see[w] = 0;
                         }
-                        if (!valid) see = 0;
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) {
-                            if (!((see >> c) & 1u)) s[c] = 0xFF800000u;
+                        for (int c = 0; c < static_cast<int>(kKvBlock); ++c) {
+                            if (!((see[c / 32] >> (c % 32)) & 1u)) s[c] = 0xFF800000u;
                         }
                     }
                     float best[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) best[i] = fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 4]));
 #pragma unroll
-                    for (int c = 8; c < 32; c += 8) {
+                    for (int c = 8; c < static_cast<int>(kKvBlock); c += 8) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             best[i] = fmaxf(fmaxf(best[i], __uint_as_float(s[c + i])), __uint_as_float(s[c + i + 4]));
                         }
                     }
-                    // The row's two threads agree on its maximum (and on whether to go on).
-                    float high = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
-                    sh.high[x][buf][half][m] = high;
-                    if (any_of(rows_id, 64, !there || !alive)) { alive = false; break; }
-                    high = fmaxf(top, fmaxf(high, sh.high[x][buf][half ^ 1u][m]));
+                    const float high = fmaxf(top, fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])));
                     // The first tokens seen, or a maximum that grew beyond what P may: a new reference.
                     const bool fresh = top == kNone;
                     const bool grow = !fresh && (high - top) * p.scale_log2 > kRescale;
                     if (__any_sync(0xffffffffu, grow)) {
-                        // (not the first step: O holds the steps before this one once they are done)
-                        if (!bar_wait(&sh.values[x], (steps_done - 1) & 1u, stop)) alive = false;
-                        alive = __all_sync(0xffffffffu, alive);     // (acted upon where both warps meet next)
-                        tmem_after_sync();
+                        // (not the first step; these scores came behind the products of the steps before)
                         const float factor = grow ? exp2_fast((top - high) * p.scale_log2) : 1.0f;
                         sum *= factor;
-                        for (uint32_t c = c_begin; c < c_end; ++c) {
+                        for (uint32_t c = 0; c < slices; ++c) {
                             uint32_t o[16];
                             tmem_load16(o_at + c * 16, o);
                             tmem_wait_load();
@@ -652,50 +647,52 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                     if (fresh || grow) top = high;
                     const float shift = top == kNone ? 0.0f : -(top * p.scale_log2);
                     const uint64_t shift2 = pair(shift, shift);
-                    uint64_t sums[2] = {0, 0};
+                    uint64_t sums[4] = {0, 0, 0, 0};
 #pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
-                        float e0, e1;
-                        unpair(fma2(pair(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), scale2, shift2), e0, e1);
-                        e0 = exp2_fast(e0);
-                        e1 = exp2_fast(e1);
-                        sums[(c / 2) % 2] = add2(sums[(c / 2) % 2], pair(e0, e1));
-                        s[c / 2] = Leaf::pack(e0, e1);
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t* const from = s + half * 64;
+#pragma unroll
+                        for (int c = 0; c < 64; c += 2) {
+                            float e0, e1;
+                            unpair(fma2(pair(__uint_as_float(from[c]), __uint_as_float(from[c + 1])), scale2, shift2), e0, e1);
+                            e0 = exp2_fast(e0);
+                            e1 = exp2_fast(e1);
+                            sums[(c / 2) % 4] = add2(sums[(c / 2) % 4], pair(e0, e1));
+                            from[c / 2] = Leaf::pack(e0, e1);
+                        }
+                        tmem_store32(s_at + half * 32, from);
+                        if (half == 1) {
+                            float a, b;
+                            unpair(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])), a, b);
+                            sum += a + b;
+                        }
+                        tmem_wait_store();
+                        tmem_before_sync();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(&sh.weights[x][half]);
                     }
-                    tmem_store16(at + half * 16, s);
-                    float a, b;
-                    unpair(add2(sums[0], sums[1]), a, b);
-                    sum += a + b;
-                    tmem_wait_store();
-                } else if (!__all_sync(0xffffffffu, there)) {
-                    alive = false;
-                    break;
+                } else {
+                    tmem_before_sync();
+                    if (lane == 0) {
+                        bar_arrive(&sh.weights[x][0]);
+                        bar_arrive(&sh.weights[x][1]);
+                    }
                 }
-                tmem_before_sync();
-                __syncwarp();
-                if (lane == 0) bar_arrive(&sh.weights[x][buf]);
             }
             if (alive && n != 0) {
-                // (a barrier of its own: when a warp comes here none, one or both of the last two steps
-                // may be done, and a parity does not tell the first case from the last)
                 alive = __all_sync(0xffffffffu, bar_wait(&sh.done[x], pieces_done & 1u, stop));
                 ++pieces_done;
                 tmem_after_sync();
             }
             // ---- results ---------------------------------------------------------------------------
-            if (busy) {
-                sh.part[x][half][m] = sum;
-                alive = !any_of(rows_id, 64, !alive);
-                sum += sh.part[x][half ^ 1u][m];
-            }
             const bool second = join && piece.steps[1] != 0;        // tile B holds part of the sum
             float mine = 1.0f, its = 0.0f;                          // factors of the two tiles' O
             if (join) {
-                if (x == 1 && half == 0) {
+                if (x == 1) {
                     sh.other[0][m] = top;
                     sh.other[1][m] = sum;
                 }
-                alive = !any_of(1, kSoftmaxWarps * 32, !alive);
+                alive = !any_of<1, kSoftmaxWarps * 32>(!alive);
                 if (x == 0 && second) {
                     const float top_b = sh.other[0][m], sum_b = sh.other[1][m];
                     const float high = fmaxf(top, top_b);
@@ -712,54 +709,57 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                 const uint64_t plane = attn_plane(p.a.out, piece.b, 0);
                 const uint32_t column = q_head * slices, local = (TREE && !p.alternate ? x * 128 : 0u) + m;
                 float* const slot = p.partial + static_cast<uint64_t>(blockIdx.x * 2 + piece.slot) * p.slot_floats;
-                for (uint32_t c = c_begin; c < c_end; ++c) {
-                    uint32_t o[16], o2[16];
-                    tmem_load16(o_at + c * 16, o);
-                    if (second) tmem_load16(o_at + 128 + c * 16, o2);
+                for (uint32_t c = 0; c < slices; c += 2) {
+                    // (32 columns at a time; those behind the head's width are not used)
+                    uint32_t o[32], o2[32];
+                    tmem_load32(o_at + c * 16, o);
+                    if (second) tmem_load32(o_at + 128 + c * 16, o2);
                     tmem_wait_load();
                     if (second) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
+                        for (int i = 0; i < 32; ++i) {
                             float v = mine == 0.0f ? 0.0f : __uint_as_float(o[i]) * mine;
                             if (its != 0.0f) v = __fmaf_rn(__uint_as_float(o2[i]), its, v);
                             o[i] = __float_as_uint(v);
                         }
                     }
-                    if (whole) {
-                        uint32_t packed[8];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float lo = __uint_as_float(o[2 * i]) * inverse, hi = __uint_as_float(o[2 * i + 1]) * inverse;
-                            bad = bad || !(fabsf(lo) <= 3.4028234e38f) || !(fabsf(hi) <= 3.4028234e38f);
-                            packed[i] = canonical_pair<Leaf>(Leaf::pack(lo, hi));
-                        }
-                        if (valid) {
-                            store_u8_stream(attn_out_piece(p.a.out, plane, row, column + c),
-                                            make_uint4(packed[0], packed[1], packed[2], packed[3]),
-                                            make_uint4(packed[4], packed[5], packed[6], packed[7]));
-                        }
-                    } else if (valid) {
-                        uint4* to = reinterpret_cast<uint4*>(slot + static_cast<uint64_t>(local) * width + c * 16);
+                    for (int half = 0; half < 2; ++half) {
+                        if (c + half >= slices) break;
+                        uint32_t* const part = o + 16 * half;
+                        if (whole) {
+                            uint32_t packed[8];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) to[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                            for (int i = 0; i < 8; ++i) {
+                                const float lo = __uint_as_float(part[2 * i]) * inverse, hi = __uint_as_float(part[2 * i + 1]) * inverse;
+                                bad = bad || !(fabsf(lo) <= 3.4028234e38f) || !(fabsf(hi) <= 3.4028234e38f);
+                                packed[i] = canonical_pair<Leaf>(Leaf::pack(lo, hi));
+                            }
+                            if (valid) {
+                                store_u8_stream(attn_out_piece(p.a.out, plane, row, column + c + half),
+                                                make_uint4(packed[0], packed[1], packed[2], packed[3]),
+                                                make_uint4(packed[4], packed[5], packed[6], packed[7]));
+                            }
+                        } else if (valid) {
+                            uint4* to = reinterpret_cast<uint4*>(slot + static_cast<uint64_t>(local) * width + (c + half) * 16);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                to[i] = make_uint4(part[4 * i], part[4 * i + 1], part[4 * i + 2], part[4 * i + 3]);
+                            }
+                        }
                     }
                 }
                 if (whole) {
-                    // Rows with a result that is not finite, in either half: once more, behind both
-                    // halves' stores.
+                    // Rows with a result that is not finite: once more, behind the stores.
                     uint32_t again = __ballot_sync(0xffffffffu, bad && valid);
-                    if (lane == 0) sh.bad[x][half][warp & 3u] = again;
-                    any_of(rows_id, 64, false);
-                    again |= sh.bad[x][half ^ 1u][warp & 3u];
-                    if (half == 0) {
-                        while (again != 0) {
-                            const int who = __ffs(again) - 1;
-                            again &= again - 1;
-                            redo_row<Leaf, TREE>(p.a, piece.b, __shfl_sync(0xffffffffu, q_head, who),
-                                                 __shfl_sync(0xffffffffu, row, who), start);
-                        }
+                    while (again != 0) {
+                        const int who = __ffs(again) - 1;
+                        again &= again - 1;
+                        __syncwarp();
+                        redo_row<Leaf, TREE>(p.a, piece.b, __shfl_sync(0xffffffffu, q_head, who),
+                                             __shfl_sync(0xffffffffu, row, who), start);
                     }
-                } else if (valid && half == 0) {
+                } else if (valid) {
                     slot[static_cast<uint64_t>(p.row_cap) * width + local] = top;
                     slot[static_cast<uint64_t>(p.row_cap) * (width + 1) + local] = sum;
                 }
@@ -767,7 +767,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             if constexpr (!TREE) break;
             tmem_before_sync();
             // Both tiles' results are out of tensor memory; one give-up ends both.
-            if (join) alive = !any_of(1, kSoftmaxWarps * 32, !alive || *stop != 0);
+            if (join) alive = !any_of<1, kSoftmaxWarps * 32>(!alive || *stop != 0);
             if (!alive) break;
             __syncwarp();
             if (lane == 0) bar_arrive(&sh.piece_free[buffer]);
@@ -775,12 +775,12 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
     } else if (run && warp == kProductWarp) {
         // ---- matrix instructions ---------------------------------------------------------------------
         const uint32_t leader = elect_lane();
-        const uint32_t kind_s = product_descriptor(Leaf::kFormat, kStep, false);
+        const uint32_t kind_s = product_descriptor(Leaf::kFormat, kKvBlock, false);
         const uint32_t kind_o = product_descriptor(Leaf::kFormat, width, true);
         const bool same_rows = TREE && p.alternate;
         const uint32_t columns = __shfl_sync(0xffffffffu, tmem, 0);
         uint32_t slot = 0, round = 0;               // next ring slot, and its phase
-        uint32_t scored[2] = {0, 0}, weighed[2] = {0, 0};       // steps of each tile, over all pieces
+        uint32_t weighed[2] = {0, 0};               // steps of each tile, over all pieces
         bool alive = true;
         auto reach = [&](uint64_t* bar, uint32_t phase, long long limit) {
             alive = __all_sync(0xffffffffu, bar_wait(bar, phase & 1u, stop, limit));
@@ -797,66 +797,94 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             const uint32_t most = max(steps0, steps1);
             const uint32_t place = TREE && p.query_buffers == 2 ? buffer : 0u;
             const uint64_t queries = operand_descriptor(q_base + place * query_bytes, 0);
-            uint32_t k_have = 0, v_have = 0, k_slot = 0, v_slot = 0;
-            auto take = [&](uint32_t& have, uint32_t& at) {
+            uint32_t k_slot = 0, v_slot = 0;
+            auto take = [&](uint32_t& at) {
                 reach(&sh.full[slot], round, kWaitCycles);
                 at = slot;
-                ++have;
                 if (++slot == p.stages) { slot = 0; ++round; }
             };
-            // S of tile x for step j = Q K^T; the caller has the step's keys.
-            auto score = [&](uint32_t x, uint32_t j) {
-                const uint32_t half = same_rows ? x : j & 1u, buf = scored[x]++ & 1u;
-                uint64_t k = operand_descriptor(ring + k_slot * block_bytes + half * (kStep * 32), 0);
+            // S of tile x = Q K^T
+            auto score = [&](uint32_t x) {
+                uint64_t k = operand_descriptor(ring + k_slot * block_bytes, 0);
                 uint64_t rows = queries + (same_rows ? 0u : x * (block_bytes >> 4));
                 for (uint32_t c = 0; c < slices; ++c) {
-                    mma_shared(leader, columns + x * 128 + buf * kStep, rows, k, kind_s, c);
+                    mma_shared(leader, columns + x * 128, rows, k, kind_s, c);
                     rows += 4096 >> 4;
                     k += 4096 >> 4;
                 }
-                mma_commit(leader, &sh.scores[x][buf]);
+                mma_commit(leader, &sh.scores[x]);
             };
-            // A block of keys (or values) is free when its last step is issued.
-            auto last_of_block = [&](uint32_t j) { return same_rows || (j & 1u) || j + 1 == most; };
-            for (uint32_t j = 0; j < 2 && j < most; ++j) {
-                if (k_have <= (same_rows ? j : 0u)) take(k_have, k_slot);
-                if (!alive) break;
-                if (j < steps0) score(0, j);
-                if (j < steps1) score(1, j);
-                if (last_of_block(j)) mma_commit(leader, &sh.empty[k_slot]);
-                if (TREE && j + 1 == most) mma_commit(leader, &sh.queries_free[place]);
-            }
-            for (uint32_t j = 0; j < most && alive; ++j) {
-                const uint32_t next = j + 2, next_block = same_rows ? next : next >> 1;
-                if (v_have <= (same_rows ? j : j >> 1)) take(v_have, v_slot);
-                if (!alive) break;
+            // O of tile x += P V, each half of P as it comes
+            auto weigh = [&](uint32_t x, uint32_t step, bool last) {
+                const uint32_t phase = weighed[x]++;
+                const uint64_t v = operand_descriptor(ring + v_slot * block_bytes, 4096);
 #pragma unroll
-                for (uint32_t x = 0; x < 2; ++x) {
-                    const uint32_t steps = x == 0 ? steps0 : steps1;
-                    if (j >= steps || !alive) continue;
-                    const uint32_t half = same_rows ? x : j & 1u, buf = weighed[x] & 1u, phase = weighed[x] >> 1;
-                    ++weighed[x];
-                    reach(&sh.weights[x][buf], phase, kWaitCycles);
-                    if (!alive) continue;
+                for (uint32_t half = 0; half < 2; ++half) {
+                    reach(&sh.weights[x][half], phase, kWaitCycles);
+                    if (!alive) return;
                     tmem_after_sync();
-                    const uint64_t v = operand_descriptor(ring + v_slot * block_bytes + half * (kStep / kTile * 512), 4096);
 #pragma unroll
-                    for (uint32_t t = 0; t < kStep / kTile; ++t) {
-                        mma_tensor(leader, columns + 256 + x * 128, columns + x * 128 + buf * kStep + t * 8,
-                                   v + t * (512 >> 4), kind_o, j + t);
-                    }
-                    mma_commit(leader, &sh.values[x]);
-                    if (j + 1 == steps) mma_commit(leader, &sh.done[x]);
-                    if (next < steps) {
-                        // (the keys two steps on come behind these values: the order of the copies)
-                        if (k_have <= next_block) take(k_have, k_slot);
-                        if (alive) score(x, next);
+                    for (uint32_t t = half * 4; t < half * 4 + 4; ++t) {
+                        mma_tensor(leader, columns + 256 + x * 128, columns + x * 128 + t * 8, v + t * (512 >> 4), kind_o, step + t);
                     }
                 }
+                if (last) mma_commit(leader, &sh.done[x]);
+            };
+            if (same_rows) {
+                // Alternate blocks: tile A the even ones, tile B the odd ones.
+#pragma unroll
+                for (uint32_t i = 0; i < 2; ++i) {
+                    if (i >= blocks || !alive) continue;
+                    take(k_slot);
+                    if (!alive) continue;
+                    score(i);
+                    mma_commit(leader, &sh.empty[k_slot]);
+                }
+                if (blocks <= 2) mma_commit(leader, &sh.queries_free[place]);
+                for (uint32_t i0 = 0; i0 < blocks && alive; i0 += 2) {
+#pragma unroll
+                    for (uint32_t x = 0; x < 2; ++x) {
+                        const uint32_t i = i0 + x;
+                        if (i >= blocks || !alive) continue;
+                        take(v_slot);
+                        if (!alive) continue;
+                        weigh(x, i0, i + 2 >= blocks);
+                        if (!alive) continue;
+                        mma_commit(leader, &sh.empty[v_slot]);
+                        if (i + 2 < blocks) {
+                            take(k_slot);
+                            if (!alive) continue;
+                            score(x);
+                            mma_commit(leader, &sh.empty[k_slot]);
+                            if (i + 3 == blocks) mma_commit(leader, &sh.queries_free[place]);
+                        }
+                    }
+                }
+            } else {
+                take(k_slot);
                 if (!alive) break;
-                if (last_of_block(j)) mma_commit(leader, &sh.empty[v_slot]);
-                if (next < most && last_of_block(next)) mma_commit(leader, &sh.empty[k_slot]);
-                if (TREE && next + 1 == most) mma_commit(leader, &sh.queries_free[place]);
+                if (steps0 != 0) score(0);
+                if (steps1 != 0) score(1);
+                mma_commit(leader, &sh.empty[k_slot]);
+                if (TREE && most == 1) mma_commit(leader, &sh.queries_free[place]);
+                for (uint32_t i = 0; i < most && alive; ++i) {
+                    take(v_slot);
+                    bool keys = false;          // (the next keys come behind these values: the order of the copies)
+#pragma unroll
+                    for (uint32_t x = 0; x < 2; ++x) {
+                        const uint32_t steps = x == 0 ? steps0 : steps1;
+                        if (i >= steps || !alive) continue;
+                        weigh(x, i, i + 1 == steps);
+                        if (!alive || i + 1 == steps) continue;
+                        if (!keys) take(k_slot);
+                        keys = true;
+                        if (alive) score(x);
+                    }
+                    if (!alive) break;
+                    mma_commit(leader, &sh.empty[v_slot]);
+                    if (keys) mma_commit(leader, &sh.empty[k_slot]);
+                    if (TREE && i + 2 == most) mma_commit(leader, &sh.queries_free[place]);
+                }
             }
             if (!TREE || !alive) break;
         }
@@ -891,7 +919,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                     ++issued;
                 };
                 const uint32_t n = piece.blocks;
-                // In the order the products take them: the keys of two steps ahead of the values.
+                // In the order the products take them: one block of keys ahead of the values, or two.
                 const uint32_t ahead = TREE && p.alternate ? 2 : 1;
                 for (uint32_t i = 0; i < ahead && i < n && alive; ++i) fetch(true, i);
                 for (uint32_t i = 0; i < n && alive; ++i) {
@@ -928,7 +956,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                 const uint32_t place = p.query_buffers == 2 ? buffer : 0u;
                 const uint32_t used = p.query_buffers == 2 ? turn / 2 : turn;      // times the place was filled
                 if (go && used > 0) alive = alive && bar_wait(&sh.queries_free[place], (used - 1) & 1u, stop, kLongWaitCycles);
-                alive = !any_of(10, kQueryThreads, !alive);     // (both warps go on or both give up)
+                alive = !any_of<2, kQueryThreads>(!alive);     // (both warps go on or both give up)
                 if (!alive) break;
                 if (me == 0) sh.pieces[buffer] = piece;
                 if (go) {
@@ -937,7 +965,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                         for (uint32_t i = me; i < piece.nodes; i += kQueryThreads) {
                             sh.parent[i] = static_cast<int16_t>(max(-1, tree_parent(parents, static_cast<int32_t>(i))));
                         }
-                        asm volatile("bar.sync 10, 64;" ::: "memory");
+                        asm volatile("bar.sync 2, 64;" ::: "memory");
                         for (uint32_t i = me; i < piece.nodes; i += kQueryThreads) {
                             uint32_t* words = sh.mask[buffer] + i * kMaskWords;
                             for (uint32_t w = 0; w < kMaskWords; ++w) words[w] = 0;
@@ -962,7 +990,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                     }
                     copies_done();
                 }
-                asm volatile("bar.sync 10, 64;" ::: "memory");
+                asm volatile("bar.sync 2, 64;" ::: "memory");
                 if (lane == 0) bar_arrive(&sh.queries[buffer]);
                 if (!go) break;
             }
