@@ -66,6 +66,12 @@ struct LeafBf16 {
     }
     // Two binary32 values to a packed pair, round to nearest even.
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
+    // x + (+0): -0 becomes +0, every finite value and infinity stays.
+    static __device__ __forceinline__ uint32_t plus_zero(uint32_t word) {
+        uint32_t r;
+        asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(word), "r"(0u));
+        return r;
+    }
     static constexpr uint32_t kNan = 0x7FC0u;
     static constexpr uint32_t kInf = 0x7F80u;
 };
@@ -77,6 +83,11 @@ struct LeafF16 {
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
         const __half2 packed = __floats2half2_rn(lo, hi);
         return *reinterpret_cast<const uint32_t*>(&packed);
+    }
+    static __device__ __forceinline__ uint32_t plus_zero(uint32_t word) {
+        uint32_t r;
+        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(word), "r"(0u));
+        return r;
     }
     static constexpr uint32_t kNan = 0x7E00u;
     static constexpr uint32_t kInf = 0x7C00u;

@@ -237,6 +237,11 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -325,8 +330,10 @@ __device__ __forceinline__ uint64_t range_begin(uint64_t total, uint32_t cta, ui
 __device__ __forceinline__ Walk plan_walk(const TcParams& p, uint32_t cta, uint32_t ctas) {
     const uint32_t lane = threadIdx.x & 31u;
     const uint32_t sets = p.a.hkv * p.pairs;
-    uint64_t total = 0;
-    for (uint32_t b = lane; b < p.a.batch; b += 32) total += tree_blocks(tree_extent(p.a, b));
+    // (the first 32 sequences, often all, are read once)
+    const uint32_t first_blocks = lane < p.a.batch ? tree_blocks(tree_extent(p.a, lane)) : 0;
+    uint64_t total = first_blocks;
+    for (uint32_t b = lane + 32; b < p.a.batch; b += 32) total += tree_blocks(tree_extent(p.a, b));
     total = warp_sum64(total) * sets;
     const uint64_t begin = range_begin(total, cta, ctas), end = range_begin(total, cta + 1, ctas);
     Walk w{0, 0, 0, end - begin};
@@ -334,7 +341,7 @@ __device__ __forceinline__ Walk plan_walk(const TcParams& p, uint32_t cta, uint3
     uint64_t before = 0;
     for (uint32_t base = 0; base < p.a.batch; base += 32) {
         const uint32_t b = base + lane;
-        const uint32_t blocks = b < p.a.batch ? tree_blocks(tree_extent(p.a, b)) : 0;
+        const uint32_t blocks = base == 0 ? first_blocks : b < p.a.batch ? tree_blocks(tree_extent(p.a, b)) : 0;
         uint64_t run = static_cast<uint64_t>(blocks) * sets;
         for (int d = 1; d < 32; d <<= 1) {
             const uint64_t up = __shfl_up_sync(0xffffffffu, run, d);
@@ -436,6 +443,7 @@ __device__ __noinline__ void redo_row(const AttnParams& p, uint32_t b, uint32_t 
 struct Shared {
     uint64_t full[kMaxStages], empty[kMaxStages];
     uint64_t scores[2], weights[2][2], done[2]; // per tile: S written, P written (halves), O complete
+    uint64_t computed[2][4];                    // per tile and warp: a step's exponentials are done
     uint64_t queries[2], queries_free[2];       // a piece's queries are there; its scores are computed
     uint64_t piece_free[2];                     // nobody reads the piece any more
     uint64_t drain;
@@ -495,6 +503,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             bar_init(&sh.weights[x][0], kSoftmaxWarps / 2);
             bar_init(&sh.weights[x][1], kSoftmaxWarps / 2);
             bar_init(&sh.done[x], 1);
+            for (uint32_t w = 0; w < 4; ++w) bar_init(&sh.computed[x][w], 1);
             bar_init(&sh.queries[x], TREE ? 2 : kSoftmaxWarps);
             bar_init(&sh.queries_free[x], 1);
             bar_init(&sh.piece_free[x], kSoftmaxWarps);
@@ -520,6 +529,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
         const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
         const bool join = TREE && p.alternate;
         uint32_t steps_done = 0, pieces_done = 0;               // of this tile, over all pieces
+        uint32_t others_done = 0;                               // steps of the other tile's pieces so far
         uint32_t head = 0, row = 0, member = m;                 // (the same in every piece while the tiles hold the same rows)
         if (join) {
             head = member / p.a.rows;
@@ -577,6 +587,14 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             const uint32_t stride = join ? 2 * kKvBlock : kKvBlock;
             // Tokens from here on may be hidden from some row of the tile.
             const uint32_t clear = TREE ? start : piece.row0 + x * p.tile_rows + 1;
+            // The two tiles' warps of one scheduler take turns with the exponentials, A first: left to
+            // themselves both compute at once, at half the rate each, and then both wait for products.
+            const uint32_t others = piece.steps[x ^ 1u];
+            auto take_turn = [&](uint32_t step) {
+                const uint32_t ahead = x == 0 ? step : step + 1;        // steps the other tile has to be through
+                if (ahead == 0 || ahead > others) return true;
+                return __all_sync(0xffffffffu, bar_wait(&sh.computed[x ^ 1u][warp & 3u], (others_done + ahead - 1) & 1u, stop)) != 0;
+            };
             for (uint32_t step = 0; step < n; ++step, ++steps_done) {
                 // (one answer per warp)
                 alive = __all_sync(0xffffffffu, bar_wait(&sh.scores[x], steps_done & 1u, stop));
@@ -645,6 +663,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                         }
                     }
                     if (fresh || grow) top = high;
+                    if (!take_turn(step)) { alive = false; break; }
                     const float shift = top == kNone ? 0.0f : -(top * p.scale_log2);
                     const uint64_t shift2 = pair(shift, shift);
                     uint64_t sums[4] = {0, 0, 0, 0};
@@ -669,16 +688,22 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                         tmem_wait_store();
                         tmem_before_sync();
                         __syncwarp();
-                        if (lane == 0) bar_arrive(&sh.weights[x][half]);
+                        if (lane == 0) {
+                            bar_arrive(&sh.weights[x][half]);
+                            if (half == 1) bar_arrive(&sh.computed[x][warp & 3u]);
+                        }
                     }
                 } else {
+                    if (!take_turn(step)) { alive = false; break; }
                     tmem_before_sync();
                     if (lane == 0) {
                         bar_arrive(&sh.weights[x][0]);
                         bar_arrive(&sh.weights[x][1]);
+                        bar_arrive(&sh.computed[x][warp & 3u]);
                     }
                 }
             }
+            others_done += others;
             if (alive && n != 0) {
                 alive = __all_sync(0xffffffffu, bar_wait(&sh.done[x], pieces_done & 1u, stop));
                 ++pieces_done;
@@ -705,42 +730,44 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             if (alive && busy && !(join && x == 1)) {
                 const bool whole = !TREE || piece.whole;
                 const float inverse = whole ? 1.0f / sum : 1.0f;
-                bool bad = !(sum > 0.0f && sum <= 3.0e38f);
                 const uint64_t plane = attn_plane(p.a.out, piece.b, 0);
                 const uint32_t column = q_head * slices, local = (TREE && !p.alternate ? x * 128 : 0u) + m;
                 float* const slot = p.partial + static_cast<uint64_t>(blockIdx.x * 2 + piece.slot) * p.slot_floats;
+                const uint64_t mine2 = pair(mine * inverse, mine * inverse), its2 = pair(its * inverse, its * inverse);
+                uint64_t zero = 0;                  // turns NaN when a result is not finite
                 for (uint32_t c = 0; c < slices; c += 2) {
                     // (32 columns at a time; those behind the head's width are not used)
                     uint32_t o[32], o2[32];
                     tmem_load32(o_at + c * 16, o);
                     if (second) tmem_load32(o_at + 128 + c * 16, o2);
                     tmem_wait_load();
-                    if (second) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            float v = mine == 0.0f ? 0.0f : __uint_as_float(o[i]) * mine;
-                            if (its != 0.0f) v = __fmaf_rn(__uint_as_float(o2[i]), its, v);
-                            o[i] = __float_as_uint(v);
-                        }
-                    }
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         if (c + half >= slices) break;
                         uint32_t* const part = o + 16 * half;
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2) {
+                            uint64_t v = mul2(pair(__uint_as_float(part[i]), __uint_as_float(part[i + 1])), mine2);
+                            if (second) {
+                                v = fma2(pair(__uint_as_float(o2[16 * half + i]), __uint_as_float(o2[16 * half + i + 1])), its2, v);
+                            }
+                            zero = fma2(v, 0, zero);
+                            float lo, hi;
+                            unpair(v, lo, hi);
+                            part[i] = __float_as_uint(lo);
+                            part[i + 1] = __float_as_uint(hi);
+                        }
+                        if (!valid) continue;
                         if (whole) {
                             uint32_t packed[8];
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
-                                const float lo = __uint_as_float(part[2 * i]) * inverse, hi = __uint_as_float(part[2 * i + 1]) * inverse;
-                                bad = bad || !(fabsf(lo) <= 3.4028234e38f) || !(fabsf(hi) <= 3.4028234e38f);
-                                packed[i] = canonical_pair<Leaf>(Leaf::pack(lo, hi));
+                                packed[i] = Leaf::plus_zero(Leaf::pack(__uint_as_float(part[2 * i]), __uint_as_float(part[2 * i + 1])));
                             }
-                            if (valid) {
-                                store_u8_stream(attn_out_piece(p.a.out, plane, row, column + c + half),
-                                                make_uint4(packed[0], packed[1], packed[2], packed[3]),
-                                                make_uint4(packed[4], packed[5], packed[6], packed[7]));
-                            }
-                        } else if (valid) {
+                            store_u8_stream(attn_out_piece(p.a.out, plane, row, column + c + half),
+                                            make_uint4(packed[0], packed[1], packed[2], packed[3]),
+                                            make_uint4(packed[4], packed[5], packed[6], packed[7]));
+                        } else {
                             uint4* to = reinterpret_cast<uint4*>(slot + static_cast<uint64_t>(local) * width + (c + half) * 16);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
@@ -749,6 +776,9 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                         }
                     }
                 }
+                float zero_lo, zero_hi;
+                unpair(zero, zero_lo, zero_hi);
+                const bool bad = !(sum > 0.0f && sum <= 3.0e38f) || zero_lo != 0.0f || zero_hi != 0.0f;
                 if (whole) {
                     // Rows with a result that is not finite: once more, behind the stores.
                     uint32_t again = __ballot_sync(0xffffffffu, bad && valid);
@@ -1067,37 +1097,40 @@ attention_join_kernel(const __grid_constant__ TcParams p, uint32_t ctas) {
         auto slot = [&](uint32_t c) {
             return p.partial + (static_cast<uint64_t>(c) * 2 + (c == c0 ? 1u : 0u)) * p.slot_floats;
         };
+        // The first ranges' values are asked for before anything else: all waits run together.
+        constexpr uint32_t kAhead = 8;
+        const uint32_t ranges = c1 - c0 + 1;
+        float v[kAhead][kMaxWidth / 32];
+        auto ask = [&](uint32_t from) {
+#pragma unroll
+            for (uint32_t i = 0; i < kAhead; ++i) {
+                const float* at = slot(c0 + min(from + i, ranges - 1)) + static_cast<uint64_t>(r) * width;
+#pragma unroll
+                for (uint32_t k = 0; k < kMaxWidth / 32; ++k) v[i][k] = lane + 32 * k < width ? at[lane + 32 * k] : 0.0f;
+            }
+        };
+        ask(0);
         float top = __int_as_float(0xFF800000);
-        for (uint32_t c = c0 + lane; c <= c1; c += 32) {
-            const float* at = slot(c);
+        for (uint32_t c = lane; c < ranges; c += 32) {
+            const float* at = slot(c0 + c);
             const float part = at[static_cast<uint64_t>(p.row_cap) * (width + 1) + r];
             const float high = at[static_cast<uint64_t>(p.row_cap) * width + r];
             if (part != 0.0f) top = fmaxf(top, high);
         }
         for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
         float sum = 0.0f, o[kMaxWidth / 32] = {};
-        for (uint32_t base = c0; base <= c1; base += 32) {
-            // Every lane has one range's factor ready; all lanes then add the ranges up in order,
-            // eight reads ahead.
+        for (uint32_t base = 0; base < ranges; base += 32) {
+            // Every lane has one range's factor ready; all lanes then add the ranges up in order.
             float factor = 0.0f, part = 0.0f;
-            if (base + lane <= c1) {
-                const float* at = slot(base + lane);
+            if (base + lane < ranges) {
+                const float* at = slot(c0 + base + lane);
                 part = at[static_cast<uint64_t>(p.row_cap) * (width + 1) + r];
                 const float high = at[static_cast<uint64_t>(p.row_cap) * width + r];
                 if (part != 0.0f) factor = exp2_fast((high - top) * p.scale_log2);
             }
-            const uint32_t count = min(32u, c1 - base + 1);
-            constexpr uint32_t kAhead = 8;
+            const uint32_t count = min(32u, ranges - base);
             for (uint32_t i0 = 0; i0 < count; i0 += kAhead) {
-                float v[kAhead][kMaxWidth / 32];
-#pragma unroll
-                for (uint32_t i = 0; i < kAhead; ++i) {
-                    const float* at = slot(base + min(i0 + i, count - 1)) + static_cast<uint64_t>(r) * width;
-#pragma unroll
-                    for (uint32_t k = 0; k < kMaxWidth / 32; ++k) {
-                        v[i][k] = lane + 32 * k < width ? at[lane + 32 * k] : 0.0f;
-                    }
-                }
+                if (base + i0 != 0) ask(base + i0);
 #pragma unroll
                 for (uint32_t i = 0; i < kAhead; ++i) {
                     const float f = __shfl_sync(0xffffffffu, factor, (i0 + i) & 31u);
