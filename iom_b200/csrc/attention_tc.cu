@@ -690,7 +690,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                         __syncwarp();
                         if (lane == 0) {
                             bar_arrive(&sh.weights[x][half]);
-                            if (half == 1) bar_arrive(&sh.computed[x][warp & 3u]);
+                            if (half == 0) bar_arrive(&sh.computed[x][warp & 3u]);
                         }
                     }
                 } else {
