@@ -569,11 +569,12 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                 // that are not there hold reaches only results nobody stores.)
                 if (valid && n != 0) {
                     const uint64_t plane = attn_plane(p.a.q, piece.b, q_head);
-                    const uint32_t dst = q_base + x * block_bytes + m * 32, flip = ((m >> 2) & 1u) * 16;
-                    for (uint32_t c = 0; c < slices; ++c) {
-                        const unsigned char* src = attn_piece(p.a.q, plane, row, c);
-                        copy16(dst + c * 4096 + flip, src);
-                        copy16(dst + c * 4096 + (16 - flip), src + 16);
+                    const unsigned char* src = attn_piece(p.a.q, plane, row, 0);
+                    uint32_t to = q_base + x * block_bytes + m * 32;
+                    const uint32_t flip = ((m >> 2) & 1u) * 16;
+                    for (uint32_t c = 0; c < slices; ++c, to += 4096, src += kTileSlots * 2) {
+                        copy16(to + flip, src);
+                        copy16(to + (16 - flip), src + 16);
                     }
                 }
                 copies_done();
@@ -1009,14 +1010,15 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                     const uint32_t offset = piece.pair * 256;
                     const uint32_t rows = min(p.alternate ? kTileRows : 2 * kTileRows, p.members - offset);
                     const uint32_t base = q_base + place * query_bytes;
-                    for (uint32_t r = me; r < rows * slices; r += kQueryThreads) {
-                        const uint32_t c = r / rows, local = r % rows, of_head = offset + local;
-                        const uint32_t q_head = piece.kv_head * p.a.group + of_head / p.a.rows;
-                        const unsigned char* src = attn_piece(p.a.q, attn_plane(p.a.q, piece.b, q_head), of_head % p.a.rows, c);
-                        const uint32_t m = local % kTileRows, flip = ((m >> 2) & 1u) * 16;
-                        const uint32_t to = base + (local / kTileRows) * block_bytes + c * 4096 + m * 32;
-                        copy16(to + flip, src);
-                        copy16(to + (16 - flip), src + 16);
+                    for (uint32_t r = me; r < rows; r += kQueryThreads) {
+                        const uint32_t of_head = offset + r, q_head = piece.kv_head * p.a.group + of_head / p.a.rows;
+                        const unsigned char* src = attn_piece(p.a.q, attn_plane(p.a.q, piece.b, q_head), of_head % p.a.rows, 0);
+                        const uint32_t m = r % kTileRows, flip = ((m >> 2) & 1u) * 16;
+                        uint32_t to = base + (r / kTileRows) * block_bytes + m * 32;
+                        for (uint32_t c = 0; c < slices; ++c, to += 4096, src += kTileSlots * 2) {
+                            copy16(to + flip, src);
+                            copy16(to + (16 - flip), src + 16);
+                        }
                     }
                     copies_done();
                 }
