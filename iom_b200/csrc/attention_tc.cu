@@ -20,21 +20,25 @@
 // What a tile's 128 rows are:
 //   packed   `pack` heads of one key/value head x 128/pack consecutive rows, so that short
 //            sequences share a tile between heads; A and B are neighbouring row blocks
-//   tree     the (head, node) pairs of one key/value head. Up to 128 pairs: both tiles hold the
-//            same rows and take alternate token blocks, joined at the end. More: A and B hold
+//   shared   a tree call with more than 128 (head, node) pairs per key/value head: A and B hold
 //            128 pairs each and share the token blocks
-// The tree call cuts the token blocks of all sequences and heads into equal ranges, one per CTA.
-// A row whose blocks lie in several ranges leaves partial (m, l, O) in the workspace and a second
-// kernel joins them, in the order of the ranges.
+//   workers  a tree call with up to 128 pairs: A and B are two workers, each with row sets, queries,
+//            ring of blocks and issuing warp of its own, so that one's change from a row set to the
+//            next (5000 clocks) runs beside the other's work. B's rows sit 32 or 64 lanes higher where
+//            they are few enough: the two then compute on different schedulers
+// A tree call cuts the token blocks of all sequences and heads into equal ranges, one per CTA or
+// worker. A row whose blocks lie in several ranges leaves partial (m, l, O) in the workspace and a
+// second kernel joins them, in the order of the ranges.
 //
 // Special rows: a row with a result that is not finite (NaN or infinities among its operands,
 // but also garbage under the mask, which the matrix instruction multiplies by zero) is computed
 // again by attend_row, which reads visible tokens only.
 //
 // Warps: 0-3 softmax of A, 4-7 softmax of B, 8 issues the matrix instructions, 9 the copies, 10
-// and 11 bring the queries of a tree call's next row set while the last one is worked on. The
-// last four hand registers to the softmax (2 x 128 x 208 + 128 x 80 of the 384 x 168 a CTA
-// starts with).
+// and 11 bring the queries of a tree call's next row set while the last one is worked on; with
+// workers 8 and 9 issue A's and B's matrix instructions, 10 and 11 their copies and queries. The
+// last four hand registers to the softmax (2 x 128 x 208 + 128 x 80 of the 384 x 168 a CTA starts
+// with).
 // Every wait is bounded; one that gives up ends all roles and is counted.
 #include <cuda.h>
 
@@ -47,7 +51,7 @@ namespace {
 
 constexpr uint32_t kThreads = 384;
 constexpr uint32_t kSoftmaxWarps = 8;
-constexpr uint32_t kProductWarp = 8, kCopyWarp = 9, kQueryWarp = 10, kQueryThreads = 64;
+constexpr uint32_t kQueryThreads = 64;
 constexpr uint32_t kTileRows = 128;
 constexpr uint32_t kMaxWidth = 128;
 constexpr uint32_t kMaxStages = 8;
@@ -70,12 +74,13 @@ struct TcParams {
     uint32_t head_tiles;        // tiles side by side: Hq / pack
     // tree
     uint32_t members;           // (head, node) pairs per key/value head
-    uint32_t alternate;         // both tiles hold the same rows
+    uint32_t lane_shift;        // workers: lanes B's rows sit higher
+    uint32_t ranges;            // of token blocks: one per CTA, or two
     uint32_t query_buffers;     // one, or two where they fit
     uint32_t pairs;             // tile pairs per key/value head
     uint32_t row_cap;           // rows of one partial
     uint64_t slot_floats;       // floats of one partial: row_cap * (D + 2), a multiple of eight
-    float* partial;             // [grid * 2][slot_floats]: O [row_cap][D], m, l
+    float* partial;             // [ranges * 2][slot_floats]: O [row_cap][D], m, l
 };
 
 // ---- barriers, copies, tensor memory ---------------------------------------------------------------
@@ -113,14 +118,12 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatil
     *stop = 1;
     return false;
 }
-// Whether any of `threads` threads says so; a barrier for them. Ids: 1 all softmax threads, 2 the
-// query warps.
-template <uint32_t id, uint32_t threads>
-__device__ __forceinline__ bool any_of(bool mine) {
+// Whether any of the query warps' threads says so; a barrier for them.
+__device__ __forceinline__ bool any_query_thread(bool mine) {
     uint32_t any;
-    asm volatile("{\n\t.reg .pred mine, any;\n\tsetp.ne.u32 mine, %3, 0;\n\t"
-                 "barrier.cta.red.or.pred any, %1, %2, mine;\n\tselp.u32 %0, 1, 0, any;\n\t}"
-                 : "=r"(any) : "n"(id), "n"(threads), "r"(mine ? 1u : 0u) : "memory");
+    asm volatile("{\n\t.reg .pred mine, any;\n\tsetp.ne.u32 mine, %2, 0;\n\t"
+                 "barrier.cta.red.or.pred any, 1, %1, mine;\n\tselp.u32 %0, 1, 0, any;\n\t}"
+                 : "=r"(any) : "n"(kQueryThreads), "r"(mine ? 1u : 0u) : "memory");
     return any != 0;
 }
 __device__ __forceinline__ void copy16(uint32_t shared, const void* global) {
@@ -253,6 +256,8 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return r;
 }
 
+enum Mode : int { kPacked, kShared, kWorkers };
+
 // ---- the work of one CTA -----------------------------------------------------------------------------
 
 // A run of token blocks of one row set (a tile pair).
@@ -296,8 +301,7 @@ __device__ __forceinline__ bool next_piece(const TcParams& p, Walk& w, Piece& ou
     out.first_token = w.block * kKvBlock;
     out.blocks = take;
     out.end = e.length + e.nodes;
-    out.steps[0] = p.alternate ? (take + 1) / 2 : take;
-    out.steps[1] = p.alternate ? take / 2 : take;
+    out.steps[0] = out.steps[1] = take;
     out.row0 = 0;
     out.start = e.length;
     out.nodes = e.nodes;
@@ -326,7 +330,7 @@ __device__ __forceinline__ uint64_t range_begin(uint64_t total, uint32_t cta, ui
     return total * cta / ctas;
 }
 
-// One warp: where this CTA's range begins.
+// One warp: where range `cta` of `ctas` begins.
 __device__ __forceinline__ Walk plan_walk(const TcParams& p, uint32_t cta, uint32_t ctas) {
     const uint32_t lane = threadIdx.x & 31u;
     const uint32_t sets = p.a.hkv * p.pairs;
@@ -444,71 +448,79 @@ struct Shared {
     uint64_t full[kMaxStages], empty[kMaxStages];
     uint64_t scores[2], weights[2][2], done[2]; // per tile: S written, P written (halves), O complete
     uint64_t computed[2][4];                    // per tile and warp: a step's exponentials are done
-    uint64_t queries[2], queries_free[2];       // a piece's queries are there; its scores are computed
-    uint64_t piece_free[2];                     // nobody reads the piece any more
-    uint64_t drain;
+    // Per worker and buffer (one worker but with kWorkers):
+    uint64_t queries[2][2], queries_free[2][2]; // a piece's queries are there; its scores are computed
+    uint64_t piece_free[2][2];                  // nobody reads the piece any more
+    uint64_t drain[2];
     uint32_t tmem, stop, run;
-    Piece pieces[2];
-    Walk walk;                                  // tree
-    float other[2][kTileRows];                  // m and l of tile B (same rows)
-    uint32_t mask[2][kMaxTreeNodes * kMaskWords];       // ancestors and the node itself
-    int16_t parent[kMaxTreeNodes];
+    Piece pieces[2][2];
+    Walk walk[2];
+    uint32_t mask[2][kMaxTreeNodes * kMaskWords];       // per buffer (workers: the first or second half of it):
+                                                        // a node's ancestors and itself
+    int16_t parent[2][kMaxTreeNodes];
 };
 
-template <class Leaf, bool TREE>
+template <class Leaf, Mode MODE>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUtensorMap k_map,
                     const __grid_constant__ CUtensorMap v_map) {
+    constexpr bool TREE = MODE != kPacked, WORKERS = MODE == kWorkers;
     extern __shared__ __align__(1024) unsigned char dynamic[];
     __shared__ Shared sh;
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31u;     // (the warp: a uniform value)
     const uint32_t width = p.a.width, slices = width / kTile;
     const uint32_t block_bytes = width * kTileRows * 2;         // a Q tile, a K block, a V block
-    const uint32_t query_bytes = (TREE && p.alternate ? 1u : 2u) * block_bytes;
-    // The dynamic part starts behind the static one: round up to the swizzle's alignment.
+    // Queries [buffer][tile], then the ring. The dynamic part starts behind the static one: round up
+    // to the swizzle's alignment.
     const uint32_t q_base = (shared_address(dynamic) + 1023u) & ~1023u;
-    const uint32_t ring = q_base + p.query_buffers * query_bytes;
+    const uint32_t ring = q_base + p.query_buffers * 2 * block_bytes;
     volatile uint32_t* const stop = &sh.stop;
 
     if (warp == 0) {
         if constexpr (TREE) {
-            const Walk w = plan_walk(p, blockIdx.x, gridDim.x);
+            const uint32_t range = WORKERS ? blockIdx.x * 2 : blockIdx.x;
+            const Walk w = plan_walk(p, range, p.ranges);
             if (lane == 0) {
-                sh.walk = w;
-                sh.run = w.left != 0;
+                sh.walk[0] = w;
+                sh.run = 1;
             }
         } else {
             Piece piece;
             bool ok;
             const bool run = plan_packed(p, blockIdx.x, piece, ok);
             if (lane == 0) {
-                sh.pieces[0] = piece;
+                sh.pieces[0][0] = piece;
                 sh.run = run;
                 if (blockIdx.x == 0) *p.a.status = ok ? 0u : 1u;
             }
         }
-    } else if (warp == kProductWarp) {
+    } else if (WORKERS && warp == 4) {
+        const Walk w = plan_walk(p, blockIdx.x * 2 + 1, p.ranges);
+        if (lane == 0) sh.walk[1] = w;
+    } else if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(shared_address(&sh.tmem)), "r"(kTmemColumns) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-    } else if (warp == kCopyWarp && lane == 0) {
+    } else if (warp == 9 && lane == 0) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&k_map)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&v_map)) : "memory");
-        for (uint32_t s = 0; s < kMaxStages; ++s) {
-            bar_init(&sh.full[s], 1);
-            bar_init(&sh.empty[s], 1);
+        for (uint32_t i = 0; i < kMaxStages; ++i) {
+            bar_init(&sh.full[i], 1);
+            bar_init(&sh.empty[i], 1);
         }
         for (uint32_t x = 0; x < 2; ++x) {
             bar_init(&sh.scores[x], 1);
-            bar_init(&sh.weights[x][0], kSoftmaxWarps / 2);
-            bar_init(&sh.weights[x][1], kSoftmaxWarps / 2);
+            bar_init(&sh.weights[x][0], 4);
+            bar_init(&sh.weights[x][1], 4);
             bar_init(&sh.done[x], 1);
             for (uint32_t w = 0; w < 4; ++w) bar_init(&sh.computed[x][w], 1);
-            bar_init(&sh.queries[x], TREE ? 2 : kSoftmaxWarps);
-            bar_init(&sh.queries_free[x], 1);
-            bar_init(&sh.piece_free[x], kSoftmaxWarps);
+            for (uint32_t i = 0; i < 2; ++i) {
+                bar_init(&sh.queries[x][i], MODE == kPacked ? kSoftmaxWarps : MODE == kShared ? 2 : 1);
+                bar_init(&sh.queries_free[x][i], 1);
+                bar_init(&sh.piece_free[x][i], WORKERS ? 4 : kSoftmaxWarps);
+            }
+            bar_init(&sh.drain[x], 1);
         }
-        bar_init(&sh.drain, 1);
         sh.stop = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -521,17 +533,81 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
     if (warp < kSoftmaxWarps) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
 
+    // A node's ancestor words. With workers a tree has at most 128 nodes: half the room each.
+    constexpr uint32_t mask_words = WORKERS ? kMaskWords / 2 : kMaskWords;
+    auto tree_mask = [&](uint32_t buffer, uint32_t worker) {
+        return sh.mask[buffer] + (WORKERS ? worker * (kMaxTreeNodes / 2) * mask_words : 0u);
+    };
+    // Publishes a piece (none: the end) with its queries and ancestor masks; `threads` threads.
+    auto bring_queries = [&](uint32_t turn, bool go, Piece& piece, uint32_t worker, uint32_t thread, uint32_t threads, bool& alive) {
+        if constexpr (TREE) {
+            auto meet = [&] {
+                if constexpr (WORKERS) __syncwarp();
+                else asm volatile("bar.sync 1, 64;" ::: "memory");
+            };
+            const uint32_t buffer = turn & 1u;
+            if (!go) piece.blocks = 0;
+            // The piece two turns back is out of use, and the queries that lie where these go.
+            if (turn >= 2) alive = bar_wait(&sh.piece_free[worker][buffer], (turn / 2 - 1) & 1u, stop, kLongWaitCycles);
+            const uint32_t place = p.query_buffers == 2 ? buffer : 0u;
+            const uint32_t used = p.query_buffers == 2 ? turn / 2 : turn;      // times the place was filled
+            if (go && used > 0) {
+                alive = alive && bar_wait(&sh.queries_free[worker][place], (used - 1) & 1u, stop, kLongWaitCycles);
+            }
+            // (all threads go on or all give up)
+            if constexpr (WORKERS) alive = __all_sync(0xffffffffu, alive);
+            else alive = !any_query_thread(!alive);
+            if (!alive) return;
+            if (thread == 0) sh.pieces[worker][buffer] = piece;
+            if (go) {
+                if (p.a.parents != nullptr && piece.first_token + piece.blocks * kKvBlock > piece.start) {
+                    const int32_t* parents = p.a.parents + static_cast<uint64_t>(piece.b) * p.a.rows;
+                    for (uint32_t i = thread; i < piece.nodes; i += threads) {
+                        sh.parent[worker][i] = static_cast<int16_t>(max(-1, tree_parent(parents, static_cast<int32_t>(i))));
+                    }
+                    meet();
+                    for (uint32_t i = thread; i < piece.nodes; i += threads) {
+                        uint32_t* words = tree_mask(buffer, worker) + i * mask_words;
+                        for (uint32_t w = 0; w < mask_words; ++w) words[w] = 0;
+                        for (int32_t at = static_cast<int32_t>(i); at >= 0; at = sh.parent[worker][at]) {
+                            words[at / 32] |= 1u << (at % 32);
+                        }
+                    }
+                }
+                // Rows of the set, 32 bytes of a tile row at a time; what the rows beside them hold
+                // reaches only results nobody stores.
+                const uint32_t offset = piece.pair * 256;
+                const uint32_t rows = min(WORKERS ? kTileRows : 2 * kTileRows, p.members - offset);
+                const uint32_t base = q_base + (place * 2 + worker) * block_bytes;
+                for (uint32_t r = thread; r < rows; r += threads) {
+                    const uint32_t of_head = offset + r, q_head = piece.kv_head * p.a.group + of_head / p.a.rows;
+                    const unsigned char* src = attn_piece(p.a.q, attn_plane(p.a.q, piece.b, q_head), of_head % p.a.rows, 0);
+                    const uint32_t at = WORKERS ? r + worker * p.lane_shift : r;
+                    const uint32_t m = at % kTileRows, flip = ((m >> 2) & 1u) * 16;
+                    uint32_t to = base + (at / kTileRows) * block_bytes + m * 32;
+                    for (uint32_t c = 0; c < slices; ++c, to += 4096, src += kTileSlots * 2) {
+                        copy16(to + flip, src);
+                        copy16(to + (16 - flip), src + 16);
+                    }
+                }
+                copies_done();
+            }
+            meet();
+            if (lane == 0) bar_arrive(&sh.queries[worker][buffer]);
+        }
+    };
+
     if (run && warp < kSoftmaxWarps) {
         // ---- softmax, one thread per row ---------------------------------------------------------------
         const uint32_t x = warp / 4, m = (warp & 3u) * 32 + lane;
         const uint32_t lanes = (warp & 3u) << 21;               // this warp's 32 tensor memory lanes
         const uint32_t s_at = tmem + lanes + x * 128, o_at = tmem + lanes + 256 + x * 128;
         const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
-        const bool join = TREE && p.alternate;
+        const uint32_t me = WORKERS ? x : 0, shift_lanes = WORKERS ? x * p.lane_shift : 0u;
         uint32_t steps_done = 0, pieces_done = 0;               // of this tile, over all pieces
         uint32_t others_done = 0;                               // steps of the other tile's pieces so far
-        uint32_t head = 0, row = 0, member = m;                 // (the same in every piece while the tiles hold the same rows)
-        if (join) {
+        uint32_t head = 0, row = 0, member = m - shift_lanes;   // (lanes below the shift: a huge number, no row)
+        if constexpr (WORKERS) {
             head = member / p.a.rows;
             row = member % p.a.rows;
         }
@@ -539,19 +615,17 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
         for (uint32_t turn = 0; ; ++turn) {
             const uint32_t buffer = TREE ? turn & 1u : 0u;
             if constexpr (TREE) {
-                alive = __all_sync(0xffffffffu, bar_wait(&sh.queries[buffer], (turn / 2) & 1u, stop, kLongWaitCycles));
-                // (one answer for all whose barriers follow)
-                if (join) alive = !any_of<1, kSoftmaxWarps * 32>(!alive);
+                alive = __all_sync(0xffffffffu, bar_wait(&sh.queries[me][buffer], (turn / 2) & 1u, stop, kLongWaitCycles));
                 if (!alive) break;
             }
-            const Piece& piece = sh.pieces[buffer];
+            const Piece& piece = sh.pieces[me][buffer];
             if (piece.blocks == 0) break;
             const uint32_t n = piece.steps[x], start = piece.start;
             // This thread's row.
             uint32_t q_head;
             bool valid;
             if constexpr (TREE) {
-                if (!join) {
+                if constexpr (!WORKERS) {
                     member = piece.pair * 256 + x * 128 + m;
                     head = member / p.a.rows;
                     row = member % p.a.rows;
@@ -579,21 +653,21 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                 }
                 copies_done();
                 __syncwarp();
-                if (lane == 0) bar_arrive(&sh.queries[0]);
+                if (lane == 0) bar_arrive(&sh.queries[0][0]);
             }
 
             const float kNone = __int_as_float(0xFF800000);
             float top = kNone, sum = 0.0f;                      // running maximum (of S) and sum
-            const uint32_t first = piece.first_token + (join ? x * kKvBlock : 0u);
-            const uint32_t stride = join ? 2 * kKvBlock : kKvBlock;
+            const uint32_t first = piece.first_token;
             // Tokens from here on may be hidden from some row of the tile.
             const uint32_t clear = TREE ? start : piece.row0 + x * p.tile_rows + 1;
             // The two tiles' warps of one scheduler take turns with the exponentials, A first: left to
             // themselves both compute at once, at half the rate each, and then both wait for products.
+            // (Workers keep no common time.)
             const uint32_t others = piece.steps[x ^ 1u];
             auto take_turn = [&](uint32_t step) {
                 const uint32_t ahead = x == 0 ? step : step + 1;        // steps the other tile has to be through
-                if (ahead == 0 || ahead > others) return true;
+                if (WORKERS || ahead == 0 || ahead > others) return true;
                 return __all_sync(0xffffffffu, bar_wait(&sh.computed[x ^ 1u][warp & 3u], (others_done + ahead - 1) & 1u, stop)) != 0;
             };
             for (uint32_t step = 0; step < n; ++step, ++steps_done) {
@@ -605,7 +679,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                     uint32_t s[kKvBlock];
 #pragma unroll
                     for (int c = 0; c < static_cast<int>(kKvBlock); c += 32) tmem_load32(s_at + c, s + c);
-                    const uint32_t token = first + step * stride;
+                    const uint32_t token = first + step * kKvBlock;
                     tmem_wait_load();
                     if (token + kKvBlock > clear || (!TREE && token < start)) {
                         uint32_t see[kKvBlock / 32];
@@ -619,13 +693,13 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                             } else {
                                 see[w] = range_word(0, static_cast<int32_t>(start) - 1 - from);
                                 const int32_t rel = from - static_cast<int32_t>(start);
-                                if (valid && rel > -32 && rel < static_cast<int32_t>(kMaxTreeNodes)) {
-                                    const uint32_t* words = sh.mask[buffer] + row * kMaskWords;
+                                if (valid && rel > -32 && rel < static_cast<int32_t>(mask_words * 32)) {
+                                    const uint32_t* words = tree_mask(buffer, x) + row * mask_words;
                                     if (rel < 0) {
                                         see[w] |= words[0] << -rel;
                                     } else {
                                         const uint32_t i = rel / 32;
-                                        see[w] |= __funnelshift_r(words[i], i + 1 < kMaskWords ? words[i + 1] : 0u, rel % 32);
+                                        see[w] |= __funnelshift_r(words[i], i + 1 < mask_words ? words[i + 1] : 0u, rel % 32);
                                     }
                                 }
                             }
@@ -711,36 +785,18 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                 tmem_after_sync();
             }
             // ---- results ---------------------------------------------------------------------------
-            const bool second = join && piece.steps[1] != 0;        // tile B holds part of the sum
-            float mine = 1.0f, its = 0.0f;                          // factors of the two tiles' O
-            if (join) {
-                if (x == 1) {
-                    sh.other[0][m] = top;
-                    sh.other[1][m] = sum;
-                }
-                alive = !any_of<1, kSoftmaxWarps * 32>(!alive);
-                if (x == 0 && second) {
-                    const float top_b = sh.other[0][m], sum_b = sh.other[1][m];
-                    const float high = fmaxf(top, top_b);
-                    mine = sum == 0.0f ? 0.0f : exp2_fast((top - high) * p.scale_log2);
-                    its = sum_b == 0.0f ? 0.0f : exp2_fast((top_b - high) * p.scale_log2);
-                    sum = sum * mine + sum_b * its;
-                    top = high;
-                }
-            }
-            if (alive && busy && !(join && x == 1)) {
+            if (alive && busy) {
                 const bool whole = !TREE || piece.whole;
                 const float inverse = whole ? 1.0f / sum : 1.0f;
                 const uint64_t plane = attn_plane(p.a.out, piece.b, 0);
-                const uint32_t column = q_head * slices, local = (TREE && !p.alternate ? x * 128 : 0u) + m;
-                float* const slot = p.partial + static_cast<uint64_t>(blockIdx.x * 2 + piece.slot) * p.slot_floats;
-                const uint64_t mine2 = pair(mine * inverse, mine * inverse), its2 = pair(its * inverse, its * inverse);
+                const uint32_t column = q_head * slices, local = WORKERS ? member : x * 128 + m;
+                float* const slot = p.partial + static_cast<uint64_t>((WORKERS ? blockIdx.x * 2 + x : blockIdx.x) * 2 + piece.slot) * p.slot_floats;
+                const uint64_t inverse2 = pair(inverse, inverse);
                 uint64_t zero = 0;                  // turns NaN when a result is not finite
                 for (uint32_t c = 0; c < slices; c += 2) {
                     // (32 columns at a time; those behind the head's width are not used)
-                    uint32_t o[32], o2[32];
+                    uint32_t o[32];
                     tmem_load32(o_at + c * 16, o);
-                    if (second) tmem_load32(o_at + 128 + c * 16, o2);
                     tmem_wait_load();
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
@@ -748,10 +804,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                         uint32_t* const part = o + 16 * half;
 #pragma unroll
                         for (int i = 0; i < 16; i += 2) {
-                            uint64_t v = mul2(pair(__uint_as_float(part[i]), __uint_as_float(part[i + 1])), mine2);
-                            if (second) {
-                                v = fma2(pair(__uint_as_float(o2[16 * half + i]), __uint_as_float(o2[16 * half + i + 1])), its2, v);
-                            }
+                            const uint64_t v = mul2(pair(__uint_as_float(part[i]), __uint_as_float(part[i + 1])), inverse2);
                             zero = fma2(v, 0, zero);
                             float lo, hi;
                             unpair(v, lo, hi);
@@ -797,19 +850,18 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             }
             if constexpr (!TREE) break;
             tmem_before_sync();
-            // Both tiles' results are out of tensor memory; one give-up ends both.
-            if (join) alive = !any_of<1, kSoftmaxWarps * 32>(!alive || *stop != 0);
             if (!alive) break;
             __syncwarp();
-            if (lane == 0) bar_arrive(&sh.piece_free[buffer]);
+            if (lane == 0) bar_arrive(&sh.piece_free[me][buffer]);
         }
-    } else if (run && warp == kProductWarp) {
+    } else if (run && (warp == 8 || (WORKERS && warp == 9))) {
         // ---- matrix instructions ---------------------------------------------------------------------
+        const uint32_t me = WORKERS ? warp - 8 : 0u;        // (workers: also the tile)
         const uint32_t leader = elect_lane();
         const uint32_t kind_s = product_descriptor(Leaf::kFormat, kKvBlock, false);
         const uint32_t kind_o = product_descriptor(Leaf::kFormat, width, true);
-        const bool same_rows = TREE && p.alternate;
         const uint32_t columns = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint32_t stages = WORKERS ? p.stages / 2 : p.stages, stage0 = WORKERS ? me * stages : 0u;
         uint32_t slot = 0, round = 0;               // next ring slot, and its phase
         uint32_t weighed[2] = {0, 0};               // steps of each tile, over all pieces
         bool alive = true;
@@ -818,26 +870,25 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
         };
         for (uint32_t turn = 0; ; ++turn) {
             const uint32_t buffer = TREE ? turn & 1u : 0u;
-            reach(&sh.queries[buffer], turn / 2, kLongWaitCycles);
+            reach(&sh.queries[me][buffer], turn / 2, kLongWaitCycles);
             if (!alive) break;
             tmem_after_sync();
-            const uint32_t blocks = __shfl_sync(0xffffffffu, sh.pieces[buffer].blocks, 0);
+            const uint32_t blocks = __shfl_sync(0xffffffffu, sh.pieces[me][buffer].blocks, 0);
             if (blocks == 0) break;
-            const uint32_t steps0 = __shfl_sync(0xffffffffu, sh.pieces[buffer].steps[0], 0);
-            const uint32_t steps1 = __shfl_sync(0xffffffffu, sh.pieces[buffer].steps[1], 0);
-            const uint32_t most = max(steps0, steps1);
+            const uint32_t steps0 = __shfl_sync(0xffffffffu, sh.pieces[me][buffer].steps[0], 0);
+            const uint32_t steps1 = __shfl_sync(0xffffffffu, sh.pieces[me][buffer].steps[1], 0);
             const uint32_t place = TREE && p.query_buffers == 2 ? buffer : 0u;
-            const uint64_t queries = operand_descriptor(q_base + place * query_bytes, 0);
+            const uint64_t queries = operand_descriptor(q_base + place * 2 * block_bytes, 0);
             uint32_t k_slot = 0, v_slot = 0;
             auto take = [&](uint32_t& at) {
-                reach(&sh.full[slot], round, kWaitCycles);
-                at = slot;
-                if (++slot == p.stages) { slot = 0; ++round; }
+                at = stage0 + slot;
+                reach(&sh.full[at], round, kWaitCycles);
+                if (++slot == stages) { slot = 0; ++round; }
             };
             // S of tile x = Q K^T
             auto score = [&](uint32_t x) {
                 uint64_t k = operand_descriptor(ring + k_slot * block_bytes, 0);
-                uint64_t rows = queries + (same_rows ? 0u : x * (block_bytes >> 4));
+                uint64_t rows = queries + x * (block_bytes >> 4);
                 for (uint32_t c = 0; c < slices; ++c) {
                     mma_shared(leader, columns + x * 128, rows, k, kind_s, c);
                     rows += 4096 >> 4;
@@ -846,8 +897,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                 mma_commit(leader, &sh.scores[x]);
             };
             // O of tile x += P V, each half of P as it comes
-            auto weigh = [&](uint32_t x, uint32_t step, bool last) {
-                const uint32_t phase = weighed[x]++;
+            auto weigh = [&](uint32_t x, uint32_t phase, uint32_t step, bool last) {
                 const uint64_t v = operand_descriptor(ring + v_slot * block_bytes, 4096);
 #pragma unroll
                 for (uint32_t half = 0; half < 2; ++half) {
@@ -861,43 +911,31 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                 }
                 if (last) mma_commit(leader, &sh.done[x]);
             };
-            if (same_rows) {
-                // Alternate blocks: tile A the even ones, tile B the odd ones.
-#pragma unroll
-                for (uint32_t i = 0; i < 2; ++i) {
-                    if (i >= blocks || !alive) continue;
+            take(k_slot);
+            if (!alive) break;
+            if constexpr (WORKERS) {
+                score(me);
+                mma_commit(leader, &sh.empty[k_slot]);
+                if (blocks == 1) mma_commit(leader, &sh.queries_free[me][place]);
+                for (uint32_t i = 0; i < blocks; ++i) {
+                    take(v_slot);
+                    if (!alive) break;
+                    weigh(me, weighed[0]++, i, i + 1 == blocks);
+                    if (!alive) break;
+                    mma_commit(leader, &sh.empty[v_slot]);
+                    if (i + 1 == blocks) break;
                     take(k_slot);
-                    if (!alive) continue;
-                    score(i);
+                    if (!alive) break;
+                    score(me);
                     mma_commit(leader, &sh.empty[k_slot]);
-                }
-                if (blocks <= 2) mma_commit(leader, &sh.queries_free[place]);
-                for (uint32_t i0 = 0; i0 < blocks && alive; i0 += 2) {
-#pragma unroll
-                    for (uint32_t x = 0; x < 2; ++x) {
-                        const uint32_t i = i0 + x;
-                        if (i >= blocks || !alive) continue;
-                        take(v_slot);
-                        if (!alive) continue;
-                        weigh(x, i0, i + 2 >= blocks);
-                        if (!alive) continue;
-                        mma_commit(leader, &sh.empty[v_slot]);
-                        if (i + 2 < blocks) {
-                            take(k_slot);
-                            if (!alive) continue;
-                            score(x);
-                            mma_commit(leader, &sh.empty[k_slot]);
-                            if (i + 3 == blocks) mma_commit(leader, &sh.queries_free[place]);
-                        }
-                    }
+                    if (i + 2 == blocks) mma_commit(leader, &sh.queries_free[me][place]);
                 }
             } else {
-                take(k_slot);
-                if (!alive) break;
+                const uint32_t most = max(steps0, steps1);
                 if (steps0 != 0) score(0);
                 if (steps1 != 0) score(1);
                 mma_commit(leader, &sh.empty[k_slot]);
-                if (TREE && most == 1) mma_commit(leader, &sh.queries_free[place]);
+                if (TREE && most == 1) mma_commit(leader, &sh.queries_free[0][place]);
                 for (uint32_t i = 0; i < most && alive; ++i) {
                     take(v_slot);
                     bool keys = false;          // (the next keys come behind these values: the order of the copies)
@@ -905,7 +943,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                     for (uint32_t x = 0; x < 2; ++x) {
                         const uint32_t steps = x == 0 ? steps0 : steps1;
                         if (i >= steps || !alive) continue;
-                        weigh(x, i, i + 1 == steps);
+                        weigh(x, weighed[x]++, i, i + 1 == steps);
                         if (!alive || i + 1 == steps) continue;
                         if (!keys) take(k_slot);
                         keys = true;
@@ -914,128 +952,91 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                     if (!alive) break;
                     mma_commit(leader, &sh.empty[v_slot]);
                     if (keys) mma_commit(leader, &sh.empty[k_slot]);
-                    if (TREE && i + 2 == most) mma_commit(leader, &sh.queries_free[place]);
+                    if (TREE && i + 2 == most) mma_commit(leader, &sh.queries_free[0][place]);
                 }
             }
             if (!TREE || !alive) break;
         }
         if (!alive) {
             // Instructions still in flight end before the tensor memory is given back.
-            mma_commit(leader, &sh.drain);
+            mma_commit(leader, &sh.drain[me]);
             const long long start = clock64();
-            while (!bar_test(&sh.drain, 0) && clock64() - start < kWaitCycles) {}
+            while (!bar_test(&sh.drain[me], 0) && clock64() - start < kWaitCycles) {}
         }
         __syncwarp();
-    } else if (run && warp == kCopyWarp) {
-        // ---- copies, one thread -----------------------------------------------------------------------------
-        if (lane == 0) {
-            uint32_t issued = 0;
-            bool alive = true;
-            Walk walk = sh.walk;
-            Piece piece = sh.pieces[0];
-            bool go = TREE ? next_piece(p, walk, piece) : true;
-            while (go && alive) {
-                const uint32_t k_plane = static_cast<uint32_t>(attn_plane(p.a.k, piece.b, piece.kv_head));
-                const uint32_t v_plane = static_cast<uint32_t>(attn_plane(p.a.v, piece.b, piece.kv_head));
-                const uint32_t first = piece.first_token / kTile;
-                auto fetch = [&](bool keys, uint32_t block) {
-                    const uint32_t slot = issued % p.stages;
-                    if (issued >= p.stages) {
-                        alive = alive && bar_wait(&sh.empty[slot], (issued / p.stages - 1) & 1u, stop, kLongWaitCycles);
-                    }
-                    if (!alive) return;
-                    bar_expect(&sh.full[slot], block_bytes);
-                    copy_block(ring + slot * block_bytes, keys ? &k_map : &v_map, &sh.full[slot],
-                               first + block * (kKvBlock / kTile), keys ? k_plane : v_plane);
-                    ++issued;
-                };
-                const uint32_t n = piece.blocks;
-                // In the order the products take them: one block of keys ahead of the values, or two.
-                const uint32_t ahead = TREE && p.alternate ? 2 : 1;
-                for (uint32_t i = 0; i < ahead && i < n && alive; ++i) fetch(true, i);
-                for (uint32_t i = 0; i < n && alive; ++i) {
-                    fetch(false, i);
-                    if (i + ahead < n && alive) fetch(true, i + ahead);
+    } else if (run && ((!WORKERS && warp == 9) || (WORKERS && warp >= 10))) {
+        // ---- copies of keys and values, one lane (workers: and the queries, all lanes) --------------------
+        const uint32_t me = WORKERS ? warp - 10 : 0u;
+        const uint32_t stages = WORKERS ? p.stages / 2 : p.stages, stage0 = WORKERS ? me * stages : 0u;
+        uint32_t issued = 0;
+        bool alive = true;
+        Walk walk = sh.walk[me];
+        Piece piece = sh.pieces[0][0];
+        for (uint32_t turn = 0; alive; ++turn) {
+            bool go = TREE ? next_piece(p, walk, piece) : turn == 0;
+            if (!WORKERS && !go) break;
+            const uint32_t k_plane = go ? static_cast<uint32_t>(attn_plane(p.a.k, piece.b, piece.kv_head)) : 0u;
+            const uint32_t v_plane = go ? static_cast<uint32_t>(attn_plane(p.a.v, piece.b, piece.kv_head)) : 0u;
+            const uint32_t first = piece.first_token / kTile;
+            auto fetch = [&](bool keys, uint32_t block) {
+                const uint32_t slot = stage0 + issued % stages;
+                if (issued >= stages) {
+                    alive = alive && bar_wait(&sh.empty[slot], (issued / stages - 1) & 1u, stop, kLongWaitCycles);
                 }
-                go = TREE ? next_piece(p, walk, piece) : false;
-            }
-            // No copy and no barrier arrival outlives the CTA.
-            const uint32_t tail = issued < p.stages ? issued : p.stages;
-            for (uint32_t i = issued - tail; i < issued; ++i) {
-                uint64_t* bar = alive ? &sh.empty[i % p.stages] : &sh.full[i % p.stages];
-                const long long start = clock64();
-                while (!bar_test(bar, (i / p.stages) & 1u) && clock64() - start < kWaitCycles) {
-                    if (alive && *stop != 0) alive = false;
-                    bar = alive ? bar : &sh.full[i % p.stages];
-                }
-            }
-        }
-        __syncwarp();
-    } else if (TREE && run) {
-        // ---- queries, pieces and ancestor masks, two warps -----------------------------------------------
-        if constexpr (TREE) {
-            const uint32_t me = threadIdx.x - kQueryWarp * 32;
-            Walk walk = sh.walk;
-            Piece piece;
-            bool alive = true;
-            for (uint32_t turn = 0; alive; ++turn) {
-                const uint32_t buffer = turn & 1u;
-                const bool go = next_piece(p, walk, piece);
-                if (!go) piece.blocks = 0;
-                // The piece two turns back is out of use, and the queries that lie where these go.
-                if (turn >= 2) alive = bar_wait(&sh.piece_free[buffer], (turn / 2 - 1) & 1u, stop, kLongWaitCycles);
-                const uint32_t place = p.query_buffers == 2 ? buffer : 0u;
-                const uint32_t used = p.query_buffers == 2 ? turn / 2 : turn;      // times the place was filled
-                if (go && used > 0) alive = alive && bar_wait(&sh.queries_free[place], (used - 1) & 1u, stop, kLongWaitCycles);
-                alive = !any_of<2, kQueryThreads>(!alive);     // (both warps go on or both give up)
+                if (!alive) return;
+                bar_expect(&sh.full[slot], block_bytes);
+                copy_block(ring + slot * block_bytes, keys ? &k_map : &v_map, &sh.full[slot],
+                           first + block * (kKvBlock / kTile), keys ? k_plane : v_plane);
+                ++issued;
+            };
+            // In the order the products take them: the keys one block ahead of the values.
+            if (go && lane == 0) fetch(true, 0);
+            if constexpr (WORKERS) {
+                alive = __all_sync(0xffffffffu, alive);
                 if (!alive) break;
-                if (me == 0) sh.pieces[buffer] = piece;
-                if (go) {
-                    if (p.a.parents != nullptr && piece.first_token + piece.blocks * kKvBlock > piece.start) {
-                        const int32_t* parents = p.a.parents + static_cast<uint64_t>(piece.b) * p.a.rows;
-                        for (uint32_t i = me; i < piece.nodes; i += kQueryThreads) {
-                            sh.parent[i] = static_cast<int16_t>(max(-1, tree_parent(parents, static_cast<int32_t>(i))));
-                        }
-                        asm volatile("bar.sync 2, 64;" ::: "memory");
-                        for (uint32_t i = me; i < piece.nodes; i += kQueryThreads) {
-                            uint32_t* words = sh.mask[buffer] + i * kMaskWords;
-                            for (uint32_t w = 0; w < kMaskWords; ++w) words[w] = 0;
-                            for (int32_t at = static_cast<int32_t>(i); at >= 0; at = sh.parent[at]) {
-                                words[at / 32] |= 1u << (at % 32);
-                            }
-                        }
-                    }
-                    // Rows of the set, 32 bytes of a tile row at a time; what the rows behind them
-                    // hold reaches only results nobody stores.
-                    const uint32_t offset = piece.pair * 256;
-                    const uint32_t rows = min(p.alternate ? kTileRows : 2 * kTileRows, p.members - offset);
-                    const uint32_t base = q_base + place * query_bytes;
-                    for (uint32_t r = me; r < rows; r += kQueryThreads) {
-                        const uint32_t of_head = offset + r, q_head = piece.kv_head * p.a.group + of_head / p.a.rows;
-                        const unsigned char* src = attn_piece(p.a.q, attn_plane(p.a.q, piece.b, q_head), of_head % p.a.rows, 0);
-                        const uint32_t m = r % kTileRows, flip = ((m >> 2) & 1u) * 16;
-                        uint32_t to = base + (r / kTileRows) * block_bytes + m * 32;
-                        for (uint32_t c = 0; c < slices; ++c, to += 4096, src += kTileSlots * 2) {
-                            copy16(to + flip, src);
-                            copy16(to + (16 - flip), src + 16);
-                        }
-                    }
-                    copies_done();
-                }
-                asm volatile("bar.sync 2, 64;" ::: "memory");
-                if (lane == 0) bar_arrive(&sh.queries[buffer]);
-                if (!go) break;
+                bring_queries(turn, go, piece, me, lane, 32u, alive);
+                if (!alive || !go) break;
             }
+            if (lane == 0) {
+                for (uint32_t i = 0; i < piece.blocks && alive; ++i) {
+                    fetch(false, i);
+                    if (i + 1 < piece.blocks && alive) fetch(true, i + 1);
+                }
+            }
+            alive = __all_sync(0xffffffffu, alive);
+        }
+        // No copy and no barrier arrival outlives the CTA.
+        if (lane == 0) {
+            const uint32_t tail = issued < stages ? issued : stages;
+            for (uint32_t i = issued - tail; i < issued; ++i) {
+                const uint32_t slot = stage0 + i % stages;
+                const long long start = clock64();
+                bool normal = alive;
+                while (!bar_test(normal ? &sh.empty[slot] : &sh.full[slot], (i / stages) & 1u) && clock64() - start < kWaitCycles) {
+                    if (*stop != 0) normal = false;
+                }
+            }
+        }
+        __syncwarp();
+    } else if (MODE == kShared && run && warp >= 10) {
+        // ---- queries, pieces and ancestor masks, two warps -----------------------------------------------
+        Walk walk = sh.walk[0];
+        Piece piece;
+        bool alive = true;
+        for (uint32_t turn = 0; alive; ++turn) {
+            const bool go = next_piece(p, walk, piece);
+            bring_queries(turn, go, piece, 0, threadIdx.x - 320, kQueryThreads, alive);
+            if (!go) break;
         }
     }
     if constexpr (TREE) {
         // (behind the copies, beside the last products)
-        if (warp == kCopyWarp && blockIdx.x == 0) warp_report_tree(p.a);
+        if (warp == 9 && blockIdx.x == 0) warp_report_tree(p.a);
     }
     tmem_before_sync();
     __syncthreads();
     tmem_after_sync();
-    if (warp == kProductWarp) {
+    if (warp == 8) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns));
         if (lane == 0 && sh.stop != 0) atomicAdd(&g_attention_timeouts, 1u);
     }
@@ -1047,7 +1048,8 @@ constexpr uint32_t kJoinWarps = 4, kJoinRows = kJoinWarps;     // rows per CTA: 
 
 template <class Leaf>
 __global__ void __launch_bounds__(kJoinWarps * 32)
-attention_join_kernel(const __grid_constant__ TcParams p, uint32_t ctas) {
+attention_join_kernel(const __grid_constant__ TcParams p) {
+    const uint32_t ctas = p.ranges;
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const uint32_t sets = p.a.hkv * p.pairs;
     const uint32_t b = blockIdx.x / sets, set = blockIdx.x % sets;
@@ -1204,32 +1206,32 @@ bool make_block_map(CUtensorMap* map, const AttnOperand& o) {
 
 // The tree call's shape: which rows share a tile, how many ranges.
 struct TreeShape {
-    uint32_t members, alternate, pairs, row_cap, ctas;
+    uint32_t members, workers, pairs, row_cap, ctas, ranges;
     bool cut;               // a row set's blocks may lie in several ranges
     uint64_t slot_floats;
 };
 TreeShape tree_shape(const AttnParams& a) {
     TreeShape t{};
     t.members = a.group * a.rows;
-    t.alternate = t.members <= kTileRows ? 1u : 0u;
-    t.pairs = t.alternate ? 1 : (t.members + 2 * kTileRows - 1) / (2 * kTileRows);
+    t.workers = t.members <= kTileRows ? 1u : 0u;
+    t.pairs = t.workers ? 1 : (t.members + 2 * kTileRows - 1) / (2 * kTileRows);
     t.row_cap = t.members < 2 * kTileRows ? t.members : 2 * kTileRows;
     const uint64_t blocks = (static_cast<uint64_t>(a.cache_rows) + kKvBlock - 1) / kKvBlock;
     const uint64_t all = static_cast<uint64_t>(a.batch) * a.hkv * t.pairs * blocks;
     t.ctas = grid_for(all, 1);
+    t.ranges = t.workers ? 2 * t.ctas : t.ctas;
     t.cut = blocks > 1;
     t.slot_floats = (static_cast<uint64_t>(t.row_cap) * (a.width + 2) + 7) / 8 * 8;
     return t;
 }
 
-// Dynamic shared memory: the queries (one tile where both hold the same rows; a second buffer where
-// it fits) and the ring of key and value blocks.
-uint32_t shared_bytes(const AttnParams& a, TcParams* p) {
+// Dynamic shared memory: the queries of two tiles (a second buffer where it fits and a tree call can
+// use it) and the ring of key and value blocks.
+uint32_t shared_bytes(const AttnParams& a, bool tree, TcParams* p) {
     const uint32_t block = a.width * kTileRows * 2;
-    const uint32_t queries = (p->alternate ? 1u : 2u) * block;
-    p->stages = kRingBytes / block < kMaxStages ? kRingBytes / block : kMaxStages;
-    p->query_buffers = queries <= 32 * 1024 ? 2 : 1;
-    return 1024 + p->query_buffers * queries + p->stages * block;
+    p->stages = (kRingBytes / block < kMaxStages ? kRingBytes / block : kMaxStages) / 2 * 2;
+    p->query_buffers = tree && 2 * block <= 32 * 1024 ? 2 : 1;
+    return 1024 + (p->query_buffers * 2 + p->stages) * block;
 }
 
 }  // namespace
@@ -1241,19 +1243,19 @@ bool attention_tc_takes(const AttnParams& p) {
 uint64_t attention_tc_workspace(const AttnParams& a) {
     const TreeShape t = tree_shape(a);
     if (!t.cut) return 0;
-    return static_cast<uint64_t>(t.ctas) * 2 * t.slot_floats * sizeof(float);
+    return static_cast<uint64_t>(t.ranges) * 2 * t.slot_floats * sizeof(float);
 }
 
-template <class Leaf, bool TREE>
+template <class Leaf, Mode MODE>
 static int launch_leaf(TcParams& p, uint32_t grid, uint32_t dynamic, const TreeShape* shape, cudaStream_t stream) {
     CUtensorMap k_map, v_map;
     if (!make_block_map(&k_map, p.a.k) || !make_block_map(&v_map, p.a.v)) {
         return fail(IOMB_ERR_DEVICE, "attention: the tensor map could not be encoded");
     }
-    const int rc = allow_full_shared_memory(reinterpret_cast<const void*>(&attention_tc_kernel<Leaf, TREE>));
+    const int rc = allow_full_shared_memory(reinterpret_cast<const void*>(&attention_tc_kernel<Leaf, MODE>));
     if (rc != IOMB_OK) return rc;
-    attention_tc_kernel<Leaf, TREE><<<grid, kThreads, dynamic, stream>>>(p, k_map, v_map);
-    if constexpr (TREE) {
+    attention_tc_kernel<Leaf, MODE><<<grid, kThreads, dynamic, stream>>>(p, k_map, v_map);
+    if constexpr (MODE != kPacked) {
         if (shape->cut) {
             const int status = check_launch("sdpa_tree launch");
             if (status != IOMB_OK) return status;
@@ -1267,12 +1269,12 @@ static int launch_leaf(TcParams& p, uint32_t grid, uint32_t dynamic, const TreeS
             early.val.programmaticStreamSerializationAllowed = 1;
             config.attrs = &early;
             config.numAttrs = 1;
-            if (cudaLaunchKernelEx(&config, attention_join_kernel<Leaf>, static_cast<const TcParams&>(p), grid) != cudaSuccess) {
+            if (cudaLaunchKernelEx(&config, attention_join_kernel<Leaf>, static_cast<const TcParams&>(p)) != cudaSuccess) {
                 return check_launch("sdpa_tree join launch");
             }
         }
     }
-    return check_launch(TREE ? "sdpa_tree launch" : "sdpa_packed launch");
+    return check_launch(MODE != kPacked ? "sdpa_tree launch" : "sdpa_packed launch");
 }
 
 int launch_attention_tc(const AttnParams& a, bool tree, bool bf16, void* workspace, cudaStream_t stream) {
@@ -1282,14 +1284,19 @@ int launch_attention_tc(const AttnParams& a, bool tree, bool bf16, void* workspa
     if (tree) {
         const TreeShape t = tree_shape(a);
         p.members = t.members;
-        p.alternate = t.alternate;
+        p.ranges = t.ranges;
+        p.lane_shift = t.members <= 32 ? 32 : t.members <= 64 ? 64 : 0;
         p.pairs = t.pairs;
         p.row_cap = t.row_cap;
         p.slot_floats = t.slot_floats;
         p.partial = static_cast<float*>(workspace);
-        const uint32_t dynamic = shared_bytes(a, &p);
-        return bf16 ? launch_leaf<LeafBf16, true>(p, t.ctas, dynamic, &t, stream)
-                    : launch_leaf<LeafF16, true>(p, t.ctas, dynamic, &t, stream);
+        const uint32_t dynamic = shared_bytes(a, true, &p);
+        if (t.workers) {
+            return bf16 ? launch_leaf<LeafBf16, kWorkers>(p, t.ctas, dynamic, &t, stream)
+                        : launch_leaf<LeafF16, kWorkers>(p, t.ctas, dynamic, &t, stream);
+        }
+        return bf16 ? launch_leaf<LeafBf16, kShared>(p, t.ctas, dynamic, &t, stream)
+                    : launch_leaf<LeafF16, kShared>(p, t.ctas, dynamic, &t, stream);
     }
     // As many heads of a group per tile as divide it, up to eight (16 rows each): heads of one
     // group read the same tokens, and short sequences fill the tile.
@@ -1302,16 +1309,18 @@ int launch_attention_tc(const AttnParams& a, bool tree, bool bf16, void* workspa
     const uint64_t units = (static_cast<uint64_t>(a.rows) / (2 * p.tile_rows) + (a.batch < a.rows ? a.batch : a.rows))
             * p.head_tiles;
     if (units > 0x7FFFFFFFull) return fail(IOMB_ERR_UNSUPPORTED, "sdpa_packed: too many rows for one launch");
-    const uint32_t dynamic = shared_bytes(a, &p);
-    return bf16 ? launch_leaf<LeafBf16, false>(p, static_cast<uint32_t>(units), dynamic, nullptr, stream)
-                : launch_leaf<LeafF16, false>(p, static_cast<uint32_t>(units), dynamic, nullptr, stream);
+    const uint32_t dynamic = shared_bytes(a, false, &p);
+    return bf16 ? launch_leaf<LeafBf16, kPacked>(p, static_cast<uint32_t>(units), dynamic, nullptr, stream)
+                : launch_leaf<LeafF16, kPacked>(p, static_cast<uint32_t>(units), dynamic, nullptr, stream);
 }
 
 int prepare_attention_kernels() {
-    for (const void* kernel : {reinterpret_cast<const void*>(&attention_tc_kernel<LeafBf16, true>),
-                               reinterpret_cast<const void*>(&attention_tc_kernel<LeafF16, true>),
-                               reinterpret_cast<const void*>(&attention_tc_kernel<LeafBf16, false>),
-                               reinterpret_cast<const void*>(&attention_tc_kernel<LeafF16, false>)}) {
+    for (const void* kernel : {reinterpret_cast<const void*>(&attention_tc_kernel<LeafBf16, kPacked>),
+                               reinterpret_cast<const void*>(&attention_tc_kernel<LeafF16, kPacked>),
+                               reinterpret_cast<const void*>(&attention_tc_kernel<LeafBf16, kShared>),
+                               reinterpret_cast<const void*>(&attention_tc_kernel<LeafF16, kShared>),
+                               reinterpret_cast<const void*>(&attention_tc_kernel<LeafBf16, kWorkers>),
+                               reinterpret_cast<const void*>(&attention_tc_kernel<LeafF16, kWorkers>)}) {
         const int rc = allow_full_shared_memory(kernel);
         if (rc != IOMB_OK) return rc;
     }
