@@ -15,7 +15,8 @@
 // The library's 16x16 tiles feed the matrix instructions without any re-layout: a tile row is 32
 // bytes, so a column of tiles is a K-major operand with 32-byte swizzle and K = 16 (one
 // instruction) for Q and K, and the same bytes are the MN-major operand of V. One tensor-map
-// copy per block fetches 128 tokens x D as [D/16][8 tiles][16][32 B].
+// copy per block fetches 128 tokens x D as [D/16][8 tiles][16][32 B], the tokens in an order of
+// their own (block_order).
 //
 // What a tile's 128 rows are:
 //   packed   `pack` heads of one key/value head x 128/pack consecutive rows, so that short
@@ -433,6 +434,18 @@ __device__ __forceinline__ uint32_t range_word(int32_t low, int32_t high) {
     return up & down;
 }
 
+// Bits of 32 tokens in the order in which the operands hold them. The copy's 128-byte swizzle is an
+// exclusive-or of address bits 4, 5, 6 with bits 7, 8, 9; inside [tile row][16 rows][32 bytes] these are
+// the 16-byte half and bits 0, 1 of the row with bits 2, 3 of the row and bit 0 of the tile row. The
+// first is the 32-byte swizzle the matrix instruction undoes. The other two permute the rows of a
+// tile, for K and V alike: products and sums do not change, but the token of a column of S does.
+__device__ __forceinline__ uint32_t block_order(uint32_t tokens) {
+    // rows 8-15 of each tile: bit 0 of the row flips
+    uint32_t w = (tokens & 0x00FF00FFu) | ((tokens & 0x55005500u) << 1) | ((tokens >> 1) & 0x55005500u);
+    // odd tile rows: bit 1 flips
+    return (w & 0x0000FFFFu) | ((w & 0x33330000u) << 2) | ((w >> 2) & 0x33330000u);
+}
+
 // attend_row for one row of a tree or packed call, out of line: rare.
 template <class Leaf, bool TREE>
 __device__ __noinline__ void redo_row(const AttnParams& p, uint32_t b, uint32_t h, uint32_t row, uint32_t start) {
@@ -703,7 +716,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                                     }
                                 }
                             }
-                            if (!valid) see[w] = 0;
+                            see[w] = valid ? block_order(see[w]) : 0u;
                         }
 #pragma unroll
                         for (int c = 0; c < static_cast<int>(kKvBlock); ++c) {
@@ -1074,21 +1087,21 @@ attention_join_kernel(const __grid_constant__ TcParams p) {
     }
     const TreeExtent e = tree_extent(p.a, b);
     const uint32_t blocks = tree_blocks(e);
-    // (every CTA waits, also one with nothing to do: the join ends after the ranges)
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (blocks == 0) return;
     total *= sets;
     const uint64_t first = before * sets + static_cast<uint64_t>(set) * blocks, end = first + blocks;
     // The ranges that hold block `first` and block `end - 1`.
     auto owner = [&](uint64_t block) {
+        if (total == 0) return 0u;
         uint32_t c = static_cast<uint32_t>(total < (1u << 22) && ctas < 1024
                 ? static_cast<uint32_t>(block) * ctas / static_cast<uint32_t>(total) : block * ctas / total);
         while (c + 1 < ctas && range_begin(total, c + 1, ctas) <= block) ++c;
         while (c > 0 && range_begin(total, c, ctas) > block) --c;
         return c;
     };
-    const uint32_t c0 = owner(first), c1 = owner(end - 1);
-    if (c0 == c1) return;                       // one range wrote the result itself
+    const uint32_t c0 = owner(first), c1 = owner(blocks != 0 ? end - 1 : first);
+    // (every CTA waits, also one with nothing to do: the join ends after the ranges)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (c0 == c1) return;                       // no blocks, or one range wrote the result itself
     const uint32_t width = p.a.width;
     const uint32_t kv_head = set / p.pairs, offset = (set % p.pairs) * 256;
     const uint32_t rows = min(p.row_cap, p.members - offset);
@@ -1189,18 +1202,21 @@ EncodeTiled encode_tiled() {
     return entry;
 }
 
-// The owner's storage as (column in tile, row in tile, tile row, tile column, plane): a box of
-// eight tile rows and every tile column lands as [tile column][tile row][16][32 bytes].
+// The owner's storage as (64 values of a tile, its four such lines, tile row, tile column, plane): a
+// box of eight tile rows and every tile column lands as [tile column][tile row][512 bytes] with the
+// 128-byte swizzle (see block_order). Lines of 128 bytes because the copy engine works line by line:
+// with the 32-byte lines that the operands' own swizzle allows it brought 20 bytes a clock and SM,
+// and head widths of 128 waited for it.
 bool make_block_map(CUtensorMap* map, const AttnOperand& o) {
     const EncodeTiled encode = encode_tiled();
     if (encode == nullptr) return false;
     const uint64_t tile_bytes = kTileSlots * 2, band_bytes = o.tile_cols * tile_bytes;
-    const cuuint64_t dims[5] = {kTile, kTile, o.tile_rows, o.tile_cols, o.planes};
-    const cuuint64_t strides[4] = {kTile * 2, band_bytes, tile_bytes, o.tile_rows * band_bytes};
-    const cuuint32_t box[5] = {kTile, kTile, kKvBlock / kTile, o.tile_cols, 1};
+    const cuuint64_t dims[5] = {64, 4, o.tile_rows, o.tile_cols, o.planes};
+    const cuuint64_t strides[4] = {128, band_bytes, tile_bytes, o.tile_rows * band_bytes};
+    const cuuint32_t box[5] = {64, 4, kKvBlock / kTile, o.tile_cols, 1};
     const cuuint32_t element_strides[5] = {1, 1, 1, 1, 1};
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, o.base, dims, strides, box, element_strides,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_32B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
