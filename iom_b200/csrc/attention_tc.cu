@@ -55,8 +55,8 @@ constexpr uint32_t kSoftmaxWarps = 8;
 constexpr uint32_t kQueryThreads = 64;
 constexpr uint32_t kTileRows = 128;
 constexpr uint32_t kMaxWidth = 128;
-constexpr uint32_t kMaxStages = 8;
-constexpr uint32_t kRingBytes = 128 * 1024;
+constexpr uint32_t kMaxStages = 12;
+constexpr uint32_t kDynamicBytes = 227 * 1024 - 20 * 1024;        // beside the static part
 constexpr uint32_t kTmemColumns = 512;          // S of A and B: 0, 128; O of A and B: 256, 384
 constexpr uint32_t kMaskWords = kMaxTreeNodes / 32;
 constexpr float kRescale = 8.0f;                // in powers of two
@@ -1245,8 +1245,9 @@ TreeShape tree_shape(const AttnParams& a) {
 // use it) and the ring of key and value blocks.
 uint32_t shared_bytes(const AttnParams& a, bool tree, TcParams* p) {
     const uint32_t block = a.width * kTileRows * 2;
-    p->stages = (kRingBytes / block < kMaxStages ? kRingBytes / block : kMaxStages) / 2 * 2;
     p->query_buffers = tree && 2 * block <= 32 * 1024 ? 2 : 1;
+    const uint32_t room = (kDynamicBytes - 1024) / block - 2 * p->query_buffers;
+    p->stages = (room < kMaxStages ? room : kMaxStages) / 2 * 2;
     return 1024 + (p->query_buffers * 2 + p->stages) * block;
 }
 
