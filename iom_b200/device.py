@@ -465,6 +465,9 @@ class SubmissionFaults:
     def clear(self) -> None:
         self._armed.clear()
 
+    def armed(self) -> bool:
+        return bool(self._armed)
+
     def take(self, point: str) -> bool:
         """True exactly once per arming, on the passage the arming named."""
         left = self._armed.get(point)
@@ -584,6 +587,8 @@ class B200Queue:
         self._lib = device._lib
         self._queue_id = queue_id
         self._stream = torch.cuda.Stream(device=device.torch_device)
+        self._stream_address = self._stream.cuda_stream
+        self._credits = device.queue_config.max_in_flight_per_queue
         self._sequence = 0
         self._records = {}        # sequence -> (event, owners, status cell or None)
         self._failures = {}       # sequence -> exception
@@ -642,11 +647,12 @@ class B200Queue:
             if not event.query():
                 event.synchronize()
             self._events.append(event)
-        if self.faults.take("complete"):
+        if self.faults.armed() and self.faults.take("complete"):
             self._failures[sequence] = DeviceError("injected completion failure")
             return
-        cells = status_cell if isinstance(status_cell, list) else \
-            ([] if status_cell is None else [status_cell])
+        if status_cell is None:
+            return
+        cells = status_cell if isinstance(status_cell, list) else [status_cell]
         if any(int(cell.item()) != 0 for cell in cells):
             self._failures[sequence] = ValueError("embedding index is negative or out of range")
 
@@ -654,31 +660,41 @@ class B200Queue:
         if self._capture is not None:
             return self._submit_captured(launch, owners, status_cell)
         try:
-            self._retire(self._device.queue_config.max_in_flight_per_queue)
-            with torch.cuda.device(self._device.ordinal):
-                if self.faults.take("launch"):
-                    raise DeviceError("injected launch failure")
-                status = launch(self._stream.cuda_stream)
-                if status != 0:
-                    raise _status_to_exception(status)
-                event = None
-                if not self.faults.take("record"):
-                    # (an event that was waited for is free again; at most one per credit exists)
-                    event = self._events.pop() if self._events else torch.cuda.Event()
-                    event.record(self._stream)
-                pinned = None
-                if status_cell is not None:
-                    slot = (self._sequence + 1) % self._status_cells.numel()
-                    pinned = self._status_cells[slot:slot + 1]
-                    with torch.cuda.stream(self._stream):
-                        pinned.copy_(status_cell, non_blocking=True)
-                    event = torch.cuda.Event()
-                    event.record(self._stream)
+            if len(self._records) >= self._credits:
+                self._retire(self._credits)
+            if torch.cuda.current_device() == self._device.ordinal:
+                event, pinned = self._issue(launch, status_cell)
+            else:
+                with torch.cuda.device(self._device.ordinal):
+                    event, pinned = self._issue(launch, status_cell)
             self._sequence += 1
             self._records[self._sequence] = (event, owners, pinned)
             return (self._queue_id << _SEQUENCE_BITS) | self._sequence
         except BaseException as error:  # the facade is noexcept: map to an oid
             return _exception_to_oid(error)
+
+    def _issue(self, launch, status_cell):
+        """The device part of _submit, on the queue's device: (completion event, pinned cell)."""
+        faults = self.faults.armed()
+        if faults and self.faults.take("launch"):
+            raise DeviceError("injected launch failure")
+        status = launch(self._stream_address)
+        if status != 0:
+            raise _status_to_exception(status)
+        event = None
+        if not (faults and self.faults.take("record")):
+            # (an event that was waited for is free again; at most one per credit exists)
+            event = self._events.pop() if self._events else torch.cuda.Event()
+            event.record(self._stream)
+        if status_cell is None:
+            return event, None
+        slot = (self._sequence + 1) % self._status_cells.numel()
+        pinned = self._status_cells[slot:slot + 1]
+        with torch.cuda.stream(self._stream):
+            pinned.copy_(status_cell, non_blocking=True)
+        event = torch.cuda.Event()
+        event.record(self._stream)
+        return event, pinned
 
     # -- CUDA graph capture ---------------------------------------------------
     def _submit_captured(self, launch, owners, status_cell) -> int:
@@ -1035,10 +1051,16 @@ class B200Queue:
     # values do not fit. They are read when the operation runs.
     def _operands(self, what: str, *views):
         """The ABI snapshots of an operation's views (None stays None)."""
+        device = self._device
+        references = []
         for view in views:
-            if view is not None:
+            if view is None:
+                references.append(None)
+                continue
+            if getattr(view.owner, "device", None) is not device:
                 self._check_view(view, what)
-        return [None if view is None else view.abi_reference() for view in views]
+            references.append(view.abi_reference())
+        return references
 
     def sdpa_packed(self, q: TensorView, k: TensorView, v: TensorView, out: TensorView,
                     offsets: int, sequences: int, status: int, scale: Optional[float] = None) -> int:
