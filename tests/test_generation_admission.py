@@ -72,6 +72,19 @@ def test_tree(change, code):
     assert _abi.last_error()
 
 
+def test_tree_workspace_is_checked():
+    lib = _abi.load_library()
+    nbytes = ctypes.c_uint64()
+    assert lib.iomb_sdpa_tree_workspace_bytes(ref(tensor((3, 4, 5, 64))), ref(tensor((3, 2, 400, 64))), ctypes.byref(nbytes)) == 0
+    assert nbytes.value > 0 and nbytes.value % 32 == 0
+    for change in (dict(workspace=None), dict(nbytes=nbytes.value - 1), dict(workspace=WORD + 16, nbytes=nbytes.value)):
+        assert tree(**change) == 1
+        assert "workspace" in _abi.last_error()
+    # a cache of one block is never cut, a width off the tensor cores has no partial sums
+    for k, q in ((tensor((3, 2, 128, 64)), tensor((3, 4, 5, 64))), (tensor((3, 2, 400, 40)), tensor((3, 4, 5, 40)))):
+        assert lib.iomb_sdpa_tree_workspace_bytes(ref(q), ref(k), ctypes.byref(nbytes)) == 0 and nbytes.value == 0
+
+
 def test_tree_workspace_bytes():
     lib = _abi.load_library()
     nbytes = ctypes.c_uint64()
@@ -79,6 +92,9 @@ def test_tree_workspace_bytes():
     assert lib.iomb_sdpa_tree_workspace_bytes(ref(q), ref(k), ctypes.byref(nbytes)) == 0
     assert lib.iomb_sdpa_tree_workspace_bytes(ref(q), ref(k), None) == 1
     assert lib.iomb_sdpa_tree_workspace_bytes(None, ref(k), ctypes.byref(nbytes)) == 1
+    assert lib.iomb_sdpa_tree_workspace_bytes(ref(tensor((3, 4, 5, 32))), ref(k), ctypes.byref(nbytes)) == 1
+    assert lib.iomb_sdpa_tree_workspace_bytes(ref(tensor((3, 5, 5, 64))), ref(k), ctypes.byref(nbytes)) == 1
+    assert lib.iomb_sdpa_tree_workspace_bytes(ref(tensor((3, 4, 257, 64))), ref(k), ctypes.byref(nbytes)) == 2
 
 
 def compact(k=None, v=None, lengths=WORD, accepted=WORD, width=8, counts=WORD, status=WORD):
