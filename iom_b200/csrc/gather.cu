@@ -296,18 +296,17 @@ cache_compact_kernel(const CompactParams p) {
     const uint64_t plane = operand_plane(cache, p.leading, index);
     const uint32_t elem = p.row.elem, per_vector = 16 / elem;
     const uint32_t column_items = count * elem;                  // vectors of one tile column
-    const uint64_t items = static_cast<uint64_t>(column_items) * p.row.tile_cols;
-    for (uint64_t first = 0; first < items; first += 32 * kCompactItems) {
+    const uint32_t items = column_items * p.row.tile_cols;       // (below 2^31, see the entry point)
+    for (uint32_t first = 0; first < items; first += 32 * kCompactItems) {
         uint4 value[kCompactItems];
         unsigned char* dst[kCompactItems];
         uint32_t valid[kCompactItems];
 #pragma unroll
         for (uint32_t u = 0; u < kCompactItems; ++u) {
-            const uint64_t item = first + u * 32 + lane;
+            const uint32_t item = first + u * 32 + lane;
             valid[u] = 0;
             if (item >= items) continue;
-            const uint32_t tc = static_cast<uint32_t>(item / column_items);
-            const uint32_t rest = static_cast<uint32_t>(item % column_items);
+            const uint32_t tc = item / column_items, rest = item % column_items;
             const uint32_t j = rest / elem, cv = rest % elem;
             const uint32_t from = path[j];
             const uint32_t col = tc * kTile + cv * per_vector;
@@ -613,7 +612,8 @@ extern "C" int iomb_cache_compact(const iomb_view* k, const iomb_view* v, const 
     }
     if (width == 0) return fail(IOMB_ERR_INVALID_ARGUMENT, "cache_compact: width must be nonzero");
     if (fk.bytes == 0) return fail(IOMB_ERR_UNSUPPORTED, "cache_compact: sub-byte leaves are not implemented");
-    if (width > (1u << 20) || k->dims[0] > 0xFFFFFFFFull || fk.rows > 0xFFFFFFFFull || fk.cols > 0xFFFFFFFFull) {
+    if (width > (1u << 20) || k->dims[0] > 0xFFFFFFFFull || fk.rows > 0xFFFFFFFFull || fk.cols > 0xFFFFFFFFull
+            || fk.tile_cols * fk.bytes > 0x7FFFFFFFull / width) {
         return fail(IOMB_ERR_UNSUPPORTED, "cache_compact: an extent exceeds the kernel limit");
     }
     CompactParams p{};
