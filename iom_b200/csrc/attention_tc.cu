@@ -469,7 +469,6 @@ __device__ __noinline__ void redo_row(const AttnParams& p, uint32_t b, uint32_t 
 struct Shared {
     uint64_t full[kMaxStages], empty[kMaxStages];
     uint64_t scores[2], weights[2][2], done[2]; // per tile: S written, P written (halves), O complete
-    uint64_t computed[2][4];                    // per tile and warp: a step's exponentials are done
     // Per worker and buffer (one worker but with kWorkers):
     uint64_t queries[2][2], queries_free[2][2]; // a piece's queries are there; its scores are computed
     uint64_t piece_free[2][2];                  // nobody reads the piece any more
@@ -535,7 +534,6 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             bar_init(&sh.weights[x][0], 4);
             bar_init(&sh.weights[x][1], 4);
             bar_init(&sh.done[x], 1);
-            for (uint32_t w = 0; w < 4; ++w) bar_init(&sh.computed[x][w], 1);
             for (uint32_t i = 0; i < 2; ++i) {
                 bar_init(&sh.queries[x][i], MODE == kPacked ? kSoftmaxWarps : MODE == kShared ? 2 : 1);
                 bar_init(&sh.queries_free[x][i], 1);
@@ -627,7 +625,6 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
         const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
         const uint32_t me = WORKERS ? x : 0, shift_lanes = WORKERS ? x * p.lane_shift : 0u;
         uint32_t steps_done = 0, pieces_done = 0;               // of this tile, over all pieces
-        uint32_t others_done = 0;                               // steps of the other tile's pieces so far
         uint32_t head = 0, row = 0, member = m - shift_lanes;   // (lanes below the shift: a huge number, no row)
         if constexpr (WORKERS) {
             head = member / p.a.rows;
@@ -683,15 +680,6 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             const uint32_t first = piece.first_token;
             // Tokens from here on may be hidden from some row of the tile.
             const uint32_t clear = TREE ? start : piece.row0 + x * p.tile_rows + 1;
-            // The two tiles' warps of one scheduler take turns with the exponentials, A first: left to
-            // themselves both compute at once, at half the rate each, and then both wait for products.
-            // (Workers keep no common time.)
-            const uint32_t others = piece.steps[x ^ 1u];
-            auto take_turn = [&](uint32_t step) {
-                const uint32_t ahead = x == 0 ? step : step + 1;        // steps the other tile has to be through
-                if (WORKERS || ahead == 0 || ahead > others) return true;
-                return __all_sync(0xffffffffu, bar_wait(&sh.computed[x ^ 1u][warp & 3u], (others_done + ahead - 1) & 1u, stop)) != 0;
-            };
             for (uint32_t step = 0; step < n; ++step, ++steps_done) {
                 // (one answer per warp)
                 alive = __all_sync(0xffffffffu, bar_wait(&sh.scores[x], steps_done & 1u, stop));
@@ -760,7 +748,6 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                         }
                     }
                     if (fresh || grow) top = high;
-                    if (!take_turn(step)) { alive = false; break; }
                     const float shift = top == kNone ? 0.0f : -(top * p.scale_log2);
                     const uint64_t shift2 = pair(shift, shift);
                     uint64_t sums[4] = {0, 0, 0, 0};
@@ -785,22 +772,16 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                         tmem_wait_store();
                         tmem_before_sync();
                         __syncwarp();
-                        if (lane == 0) {
-                            bar_arrive(&sh.weights[x][half]);
-                            if (half == 0) bar_arrive(&sh.computed[x][warp & 3u]);
-                        }
+                        if (lane == 0) bar_arrive(&sh.weights[x][half]);
                     }
                 } else {
-                    if (!take_turn(step)) { alive = false; break; }
                     tmem_before_sync();
                     if (lane == 0) {
                         bar_arrive(&sh.weights[x][0]);
                         bar_arrive(&sh.weights[x][1]);
-                        bar_arrive(&sh.computed[x][warp & 3u]);
                     }
                 }
             }
-            others_done += others;
             if (alive && n != 0) {
                 alive = __all_sync(0xffffffffu, bar_wait(&sh.done[x], pieces_done & 1u, stop));
                 ++pieces_done;
