@@ -80,7 +80,7 @@ struct TcParams {
     uint32_t query_buffers;     // one, or two where they fit
     uint32_t pairs;             // tile pairs per key/value head
     uint32_t row_cap;           // rows of one partial
-    uint32_t set_cost;          // see set_length
+    uint32_t set_cost, cut;     // see set_length
     uint64_t slot_floats;       // floats of one partial: row_cap * (D + 2), a multiple of eight
     float* partial;             // [ranges * 2][slot_floats]: O [row_cap][D], m, l
 };
@@ -280,10 +280,10 @@ __device__ __forceinline__ uint32_t tree_blocks(const TreeExtent& e) {
     return e.nodes == 0 ? 0 : (e.length + e.nodes + kKvBlock - 1) / kKvBlock;
 }
 // Length of a row set when ranges are cut: its blocks, behind `set_cost` more that stand for the change
-// to it from another set (queries, first scores, results).
+// to it from another set (queries, first scores, results). Where sets stay whole it is one place.
 __device__ __forceinline__ uint32_t set_length(const TcParams& p, const TreeExtent& e) {
     const uint32_t blocks = tree_blocks(e);
-    return blocks == 0 ? 0 : blocks + p.set_cost;
+    return blocks == 0 ? 0 : p.cut ? blocks + p.set_cost : 1;
 }
 
 // Walks the pieces of a range: sequences, then (head, pair), then places of the set.
@@ -302,7 +302,8 @@ __device__ __forceinline__ bool next_piece(const TcParams& p, Walk& w, Piece& ou
         }
         const uint32_t rest = length - w.place;
         const uint32_t take = w.left < rest ? static_cast<uint32_t>(w.left) : rest;
-        const uint32_t begin = max(w.place, p.set_cost) - p.set_cost, end = max(w.place + take, p.set_cost) - p.set_cost;
+        const uint32_t begin = p.cut ? max(w.place, p.set_cost) - p.set_cost : 0;
+        const uint32_t end = p.cut ? max(w.place + take, p.set_cost) - p.set_cost : blocks;
         out.b = w.b;
         out.kv_head = w.set / p.pairs;
         out.pair = w.set % p.pairs;
@@ -1222,10 +1223,14 @@ TreeShape tree_shape(const AttnParams& a) {
     t.pairs = t.workers ? 1 : (t.members + 2 * kTileRows - 1) / (2 * kTileRows);
     t.row_cap = t.members < 2 * kTileRows ? t.members : 2 * kTileRows;
     const uint64_t blocks = (static_cast<uint64_t>(a.cache_rows) + kKvBlock - 1) / kKvBlock;
-    const uint64_t all = static_cast<uint64_t>(a.batch) * a.hkv * t.pairs * blocks;
-    t.ctas = grid_for(all, 1);
+    // Short caches stay whole: cutting them saves less than the second kernel costs. One token of one
+    // sequence (four sets): caches of two blocks 9.2 us whole and 10.7 cut, of four 11.8 and 10.8 (and
+    // 2.5 us less for the host), of eight 17.1 and 11.5. 256 sets of one token: eight blocks 20.9 whole
+    // and 21.6 cut; 64 sets of 256 rows: eight blocks 26.0 and 39.4.
+    const uint64_t sets = static_cast<uint64_t>(a.batch) * a.hkv * t.pairs;
+    t.cut = blocks > (sets >= 48 ? 8 : 4);
+    t.ctas = grid_for(t.cut ? sets * blocks : sets, 1);
     t.ranges = t.workers ? 2 * t.ctas : t.ctas;
-    t.cut = blocks > 1;
     t.slot_floats = (static_cast<uint64_t>(t.row_cap) * (a.width + 2) + 7) / 8 * 8;
     return t;
 }
@@ -1291,6 +1296,7 @@ int launch_attention_tc(const AttnParams& a, bool tree, bool bf16, void* workspa
         const TreeShape t = tree_shape(a);
         p.members = t.members;
         p.ranges = t.ranges;
+        p.cut = t.cut ? 1u : 0u;
         // (decodes of 64 sequences: 31.6 us at none, 26.7 at one or two, 29.9 at five; eight trees of 64
         // nodes: 74.7 at none, 72.9 at two, 69.8 at five)
         p.set_cost = t.workers ? 2 : 5;

@@ -75,13 +75,14 @@ def test_tree(change, code):
 def test_tree_workspace_is_checked():
     lib = _abi.load_library()
     nbytes = ctypes.c_uint64()
-    assert lib.iomb_sdpa_tree_workspace_bytes(ref(tensor((3, 4, 5, 64))), ref(tensor((3, 2, 400, 64))), ctypes.byref(nbytes)) == 0
+    long = tensor((3, 2, 4000, 64))
+    assert lib.iomb_sdpa_tree_workspace_bytes(ref(tensor((3, 4, 5, 64))), ref(long), ctypes.byref(nbytes)) == 0
     assert nbytes.value > 0 and nbytes.value % 32 == 0
     for change in (dict(workspace=None), dict(nbytes=nbytes.value - 1), dict(workspace=WORD + 16, nbytes=nbytes.value)):
-        assert tree(**change) == 1
+        assert tree(k=long, v=tensor((3, 2, 4000, 64)), **change) == 1
         assert "workspace" in _abi.last_error()
-    # a cache of one block is never cut, a width off the tensor cores has no partial sums
-    for k, q in ((tensor((3, 2, 128, 64)), tensor((3, 4, 5, 64))), (tensor((3, 2, 400, 40)), tensor((3, 4, 5, 40)))):
+    # a short cache is never cut, a width off the tensor cores has no partial sums
+    for k, q in ((tensor((3, 2, 128, 64)), tensor((3, 4, 5, 64))), (tensor((3, 2, 4000, 40)), tensor((3, 4, 5, 40)))):
         assert lib.iomb_sdpa_tree_workspace_bytes(ref(q), ref(k), ctypes.byref(nbytes)) == 0 and nbytes.value == 0
 
 
