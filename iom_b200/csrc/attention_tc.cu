@@ -31,9 +31,18 @@
 // worker. A row whose blocks lie in several ranges leaves partial (m, l, O) in the workspace and a
 // second kernel joins them, in the order of the ranges.
 //
-// Special rows: a row with a result that is not finite (NaN or infinities among its operands,
-// but also garbage under the mask, which the matrix instruction multiplies by zero) is computed
-// again by attend_row, which reads visible tokens only.
+// Special rows: a row with a result that is not finite (NaN or infinities among its operands or
+// under its mask, where the matrix instruction multiplies them by zero) is computed again by
+// attend_row, which reads visible tokens only. Tiles of tokens that no row sees take no part, and
+// values beside the sequence in its first and last tile are zeroed as they arrive.
+//
+// What bounds it (one B200; rates by the algorithm's bytes and products):
+//   packed 4 x 4096 rows   32 heads on 4, D 128: 520 us, 1060 TFLOP/s. Per step of 128 x 128 scores the
+//                          exponentials take 1024 clocks of the SM's special-function units, the two
+//                          products 1024 of the tensor cores, and neither reaches beyond 53 % of the
+//                          time: what is left is the softmax's other instructions between two handovers.
+//   tree, long caches      8 trees, 427 MB of keys and values: 90 us, 4.7 TB/s
+//   tree, single tokens    64 decodes: 28 us, 2.4 TB/s; the changes between row sets and the second kernel
 //
 // Warps: 0-3 softmax of A, 4-7 softmax of B, 8 issues the matrix instructions, 9 the copies, 10
 // and 11 bring the queries of a tree call's next row set while the last one is worked on; with
@@ -268,6 +277,7 @@ struct Piece {
     uint32_t first_token;       // multiple of 16: the first block's first row of k and v
     uint32_t blocks;            // blocks of 128 tokens; none: there are no more pieces
     uint32_t steps[2];          // blocks per tile
+    uint32_t seen[2];           // tokens from first_token on, beyond which no row of the tile sees
     uint32_t end;               // rows of the sequence end here (packed), live rows (tree)
     uint32_t row0;              // packed: first row of tile A
     uint32_t start;             // packed: first row of the sequence; tree: rows before the tree
@@ -320,6 +330,7 @@ __device__ __forceinline__ bool next_piece(const TcParams& p, Walk& w, Piece& ou
         out.first_token = begin * kKvBlock;
         out.blocks = out.steps[0] = out.steps[1] = end - begin;
         out.end = e.length + e.nodes;
+        out.seen[0] = out.seen[1] = out.end - out.first_token;
         out.row0 = 0;
         out.start = e.length;
         out.nodes = e.nodes;
@@ -428,7 +439,8 @@ __device__ __forceinline__ bool plan_packed(const TcParams& p, uint32_t unit, Pi
     for (uint32_t x = 0; x < 2; ++x) {
         const uint32_t row = out.row0 + x * p.tile_rows;
         const uint32_t last = min(out.end, row + p.tile_rows);      // one behind the tile's last row
-        out.steps[x] = row < out.end ? (last - out.first_token + kKvBlock - 1) / kKvBlock : 0;
+        out.seen[x] = row < out.end ? last - out.first_token : 0;
+        out.steps[x] = (out.seen[x] + kKvBlock - 1) / kKvBlock;
     }
     out.blocks = max(out.steps[0], out.steps[1]);
     out.nodes = 0;
@@ -470,6 +482,7 @@ __device__ __noinline__ void redo_row(const AttnParams& p, uint32_t b, uint32_t 
 struct Shared {
     uint64_t full[kMaxStages], empty[kMaxStages];
     uint64_t scores[2], weights[2][2], done[2]; // per tile: S written, P written (halves), O complete
+    uint64_t landed[2];                         // per copying warp: values to be cleaned are there
     // Per worker and buffer (one worker but with kWorkers):
     uint64_t queries[2][2], queries_free[2][2]; // a piece's queries are there; its scores are computed
     uint64_t piece_free[2][2];                  // nobody reads the piece any more
@@ -541,6 +554,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                 bar_init(&sh.piece_free[x][i], WORKERS ? 4 : kSoftmaxWarps);
             }
             bar_init(&sh.drain[x], 1);
+            bar_init(&sh.landed[x], 1);
         }
         sh.stop = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -683,7 +697,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             const uint32_t clear = TREE ? start : piece.row0 + x * p.tile_rows + 1;
             for (uint32_t step = 0; step < n; ++step, ++steps_done) {
                 // (one answer per warp)
-                alive = __all_sync(0xffffffffu, bar_wait(&sh.scores[x], steps_done & 1u, stop));
+                alive = __all_sync(0xffffffffu, bar_wait(&sh.scores[x], steps_done & 1u, stop, kLongWaitCycles));
                 if (!alive) break;
                 tmem_after_sync();
                 if (busy) {
@@ -784,7 +798,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                 }
             }
             if (alive && n != 0) {
-                alive = __all_sync(0xffffffffu, bar_wait(&sh.done[x], pieces_done & 1u, stop));
+                alive = __all_sync(0xffffffffu, bar_wait(&sh.done[x], pieces_done & 1u, stop, kLongWaitCycles));
                 ++pieces_done;
                 tmem_after_sync();
             }
@@ -881,6 +895,8 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             if (blocks == 0) break;
             const uint32_t steps0 = __shfl_sync(0xffffffffu, sh.pieces[me][buffer].steps[0], 0);
             const uint32_t steps1 = __shfl_sync(0xffffffffu, sh.pieces[me][buffer].steps[1], 0);
+            const uint32_t seen0 = __shfl_sync(0xffffffffu, sh.pieces[me][buffer].seen[0], 0);
+            const uint32_t seen1 = __shfl_sync(0xffffffffu, sh.pieces[me][buffer].seen[1], 0);
             const uint32_t place = TREE && p.query_buffers == 2 ? buffer : 0u;
             const uint64_t queries = operand_descriptor(q_base + place * 2 * block_bytes, 0);
             uint32_t k_slot = 0, v_slot = 0;
@@ -900,17 +916,23 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                 }
                 mma_commit(leader, &sh.scores[x]);
             };
-            // O of tile x += P V, each half of P as it comes
+            // O of tile x += P V, each half of P as it comes; not the tiles of 16 tokens that no row sees
             auto weigh = [&](uint32_t x, uint32_t phase, uint32_t step, bool last) {
                 const uint64_t v = operand_descriptor(ring + v_slot * block_bytes, 4096);
+                const uint32_t seen = (x == 0 ? seen0 : seen1) - step * kKvBlock;
 #pragma unroll
                 for (uint32_t half = 0; half < 2; ++half) {
-                    reach(&sh.weights[x][half], phase, kWaitCycles);
+                    reach(&sh.weights[x][half], phase, kLongWaitCycles);
                     if (!alive) return;
                     tmem_after_sync();
-#pragma unroll
-                    for (uint32_t t = half * 4; t < half * 4 + 4; ++t) {
+                    auto product = [&](uint32_t t) {
                         mma_tensor(leader, columns + 256 + x * 128, columns + x * 128 + t * 8, v + t * (512 >> 4), kind_o, step + t);
+                    };
+                    if (seen >= (half + 1) * 64) {
+#pragma unroll
+                        for (uint32_t t = 0; t < 4; ++t) product(half * 4 + t);
+                    } else {
+                        for (uint32_t t = half * 4; t * kTile < seen; ++t) product(t);
                     }
                 }
                 if (last) mma_commit(leader, &sh.done[x]);
@@ -969,10 +991,10 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
         }
         __syncwarp();
     } else if (run && ((!WORKERS && warp == 9) || (WORKERS && warp >= 10))) {
-        // ---- copies of keys and values, one lane (workers: and the queries, all lanes) --------------------
+        // ---- copies of keys and values (workers: and the queries) -----------------------------------------
         const uint32_t me = WORKERS ? warp - 10 : 0u;
         const uint32_t stages = WORKERS ? p.stages / 2 : p.stages, stage0 = WORKERS ? me * stages : 0u;
-        uint32_t issued = 0;
+        uint32_t issued = 0, filled = 0, cleaned = 0;   // (filled: lane 0, copies under way or done)
         bool alive = true;
         Walk walk = sh.walk[me];
         Piece piece = sh.pieces[0][0];
@@ -982,37 +1004,64 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             const uint32_t k_plane = go ? static_cast<uint32_t>(attn_plane(p.a.k, piece.b, piece.kv_head)) : 0u;
             const uint32_t v_plane = go ? static_cast<uint32_t>(attn_plane(p.a.v, piece.b, piece.kv_head)) : 0u;
             const uint32_t first = piece.first_token / kTile;
+            // Values beside the sequence, in a tile of 16 tokens that it begins or ends in, become zeros: what
+            // such rows hold (a cache is rarely set up before use) would make every result NaN, by way of
+            // 0 x NaN, and every row be computed again, one at a time: 32 single-token decodes over caches
+            // with NaN behind the live rows took 5065 us instead of 25, and take 26 with the zeros.
+            const uint32_t lead = TREE ? 0u : piece.start - piece.first_token, live = piece.end - piece.first_token;
             auto fetch = [&](bool keys, uint32_t block) {
-                const uint32_t slot = stage0 + issued % stages;
-                if (issued >= stages) {
-                    alive = alive && bar_wait(&sh.empty[slot], (issued / stages - 1) & 1u, stop, kLongWaitCycles);
+                const uint32_t slot = stage0 + issued % stages, to = ring + slot * block_bytes;
+                const uint32_t low = block == 0 ? lead : 0u, high = min(kKvBlock, live - block * kKvBlock);
+                const bool clean = !keys && (low != 0 || high % kTile != 0);
+                if (lane == 0) {
+                    if (issued >= stages) {
+                        alive = alive && bar_wait(&sh.empty[slot], (issued / stages - 1) & 1u, stop, kLongWaitCycles);
+                    }
+                    if (alive) {
+                        uint64_t* const bar = clean ? &sh.landed[me] : &sh.full[slot];
+                        bar_expect(bar, block_bytes);
+                        copy_block(to, keys ? &k_map : &v_map, bar, first + block * (kKvBlock / kTile), keys ? k_plane : v_plane);
+                        filled = issued + 1;
+                    }
                 }
-                if (!alive) return;
-                bar_expect(&sh.full[slot], block_bytes);
-                copy_block(ring + slot * block_bytes, keys ? &k_map : &v_map, &sh.full[slot],
-                           first + block * (kKvBlock / kTile), keys ? k_plane : v_plane);
                 ++issued;
+                if (!clean) return;
+                alive = __all_sync(0xffffffffu, alive);
+                if (!alive) return;
+                alive = __all_sync(0xffffffffu, bar_wait(&sh.landed[me], cleaned++ & 1u, stop));
+                if (!alive) return;
+                // A lane per 16 bytes of a tile row's 32: of rows [0, low) and [high, the tile's end).
+                const uint32_t row = lane / 2, last = high / kTile;
+                for (uint32_t side = 0; side < 2; ++side) {
+                    if (side == 0 ? row >= low : high % kTile == 0 || row < high % kTile) continue;
+                    const uint32_t at = (side == 0 ? 0u : last * 512) + lane * 16, place = at ^ (at >> 7 & 7u) << 4;
+                    for (uint32_t c = 0; c < slices; ++c) {
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to + c * 4096 + place), "r"(0u) : "memory");
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) bar_arrive(&sh.full[slot]);
             };
             // In the order the products take them: the keys one block ahead of the values.
-            if (go && lane == 0) fetch(true, 0);
+            if (go) fetch(true, 0);
             if constexpr (WORKERS) {
                 alive = __all_sync(0xffffffffu, alive);
                 if (!alive) break;
                 bring_queries(turn, go, piece, me, lane, 32u, alive);
                 if (!alive || !go) break;
             }
-            if (lane == 0) {
-                for (uint32_t i = 0; i < piece.blocks && alive; ++i) {
-                    fetch(false, i);
-                    if (i + 1 < piece.blocks && alive) fetch(true, i + 1);
-                }
+            // (all lanes to the end, also where lane 0 gave up)
+            for (uint32_t i = 0; i < piece.blocks; ++i) {
+                fetch(false, i);
+                if (i + 1 < piece.blocks) fetch(true, i + 1);
             }
             alive = __all_sync(0xffffffffu, alive);
         }
         // No copy and no barrier arrival outlives the CTA.
         if (lane == 0) {
-            const uint32_t tail = issued < stages ? issued : stages;
-            for (uint32_t i = issued - tail; i < issued; ++i) {
+            const uint32_t tail = filled < stages ? filled : stages;
+            for (uint32_t i = filled - tail; i < filled; ++i) {
                 const uint32_t slot = stage0 + i % stages;
                 const long long start = clock64();
                 bool normal = alive;
