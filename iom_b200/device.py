@@ -644,8 +644,7 @@ class B200Queue:
         if event is None:
             self._stream.synchronize()      # no event could be recorded: drain the stream
         else:
-            if not event.query():
-                event.synchronize()
+            event.synchronize()
             self._events.append(event)
         if self.faults.armed() and self.faults.take("complete"):
             self._failures[sequence] = DeviceError("injected completion failure")
