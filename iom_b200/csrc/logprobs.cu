@@ -18,6 +18,10 @@
 // reaches it too, and only the slots whose own maximum does (about K of them) are read again for
 // their elements. The owner ranks these candidates. Rows where that breaks down (more than 256
 // candidates, which takes ties by the hundred, or NaN) are ranked by one warp that walks the row.
+//
+// Bound by HBM where there are many rows: 2045 rows of 50021 F32 logits take 73 us per call on a B200
+// (5.6 TB/s). 64 rows of 32000 BF16 take 9.3 us, bound by the chain load, cluster
+// barrier, candidates, ranking; clusters of eight put 32 CTAs on them instead of four.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
