@@ -252,3 +252,21 @@ def test_same_call_gives_the_same_bits(gpu):
     for _ in range(3):
         run(queue, case.issue(queue))
         assert np.array_equal(first, download(case.dev["out"]))
+
+
+@pytest.mark.parametrize("width", [16, 64, 80, 128])
+@pytest.mark.parametrize("first", range(0, 18, 3))
+def test_every_start_and_end_inside_a_tile(gpu, width, first):
+    """The tiles that a sequence shares with NaN rows beside it, at every offset."""
+    device, queue = gpu
+    borders = [first]
+    for n in range(1, 18):
+        borders.append(borders[-1] + 16 + n)
+
+    def edit(v):
+        for x in v.values():
+            x[:, :first] = np.nan
+            x[:, borders[-1]:] = np.nan
+    case = Packed(device, DataType.BF16, 2, 1, width, borders, rows=borders[-1] + 40, seed=first, edit=edit)
+    run(queue, case.issue(queue))
+    case.check()

@@ -279,3 +279,18 @@ def test_two_queues_at_once_and_the_same_bits(gpu):
         b.check(nodes=(0, 2), heads=(0, 7))
     finally:
         other.close()
+
+
+@pytest.mark.parametrize("width,nodes,hq", [(16, 1, 2), (64, 3, 8), (128, 2, 4), (80, 150, 2)])
+def test_every_end_inside_a_tile(gpu, width, nodes, hq):
+    """The last tile of every sequence, shared with NaN rows behind it, at every offset."""
+    device, queue = gpu
+    lengths = [n if n % 2 else 120 + n for n in range(32)] + [600, 1100, 1301]
+
+    def edit(v):
+        for b, n in enumerate(lengths):
+            v["k"][b, :, n + nodes:] = np.nan
+            v["v"][b, :, n + nodes:] = np.nan
+    case = Tree(device, DataType.BF16, hq, 1, width, nodes, 1500, lengths, seed=width, edit=edit)
+    run(queue, case.issue(queue))
+    case.check(nodes=[0, nodes - 1])
