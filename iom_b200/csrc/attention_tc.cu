@@ -1129,15 +1129,29 @@ attention_join_kernel(const __grid_constant__ TcParams p) {
     const uint32_t length = set_length(p, e);
     total *= sets;
     const uint64_t begin = before * sets + static_cast<uint64_t>(set) * length;
-    // The ranges that hold the set's first and last block.
-    auto owner = [&](uint64_t block) {
-        uint32_t c = static_cast<uint32_t>(total < (1u << 22) && ctas < 1024
-                ? static_cast<uint32_t>(block) * ctas / static_cast<uint32_t>(total) : block * ctas / total);
-        while (c + 1 < ctas && range_begin(total, c + 1, ctas) <= block) ++c;
-        while (c > 0 && range_begin(total, c, ctas) > block) --c;
-        return c;
+    // The range that holds a place: the last one that begins at or before it,
+    // total * c / ctas < place + 1.
+    auto owner = [&](uint64_t place) {
+        if (total < (1u << 22) && ctas < 1024) {        // (short division)
+            const uint32_t n = static_cast<uint32_t>(total);
+            return ((static_cast<uint32_t>(place) + 1) * ctas + n - 1) / n - 1;
+        }
+        return static_cast<uint32_t>(((place + 1) * ctas + total - 1) / total - 1);
     };
     const uint32_t c0 = length != 0 ? owner(begin + p.set_cost) : 0, c1 = length != 0 ? owner(begin + length - 1) : 0;
+    // With fewer places than ranges (short lengths in a large cache) some ranges between the two hold
+    // nothing and left their partials unwritten; those that hold something then hold one block each.
+    // (`places`: their number, or zero where there are enough; the owner's formula, in 32 bits)
+    const uint32_t places = total < ctas ? static_cast<uint32_t>(total) : 0u;
+    const uint32_t behind = static_cast<uint32_t>(begin) + p.set_cost + 1;
+    const uint32_t ranges = places != 0 && length != 0 ? length - p.set_cost : c1 - c0 + 1;
+    // The partial of the set's i-th range. (The row set began in range c0, behind its first block or
+    // at it: the second partial; the others began with it.)
+    auto partial = [&](uint32_t i) {
+        const uint32_t c = places != 0 ? ((behind + i) * ctas + places - 1) / places - 1 : c0 + i;
+        return c * 2 + (i == 0 ? 1u : 0u);
+    };
+    const uint32_t first_ready = partial(min(lane, ranges - 1));
     // (every CTA waits, also one with nothing to do: the join ends after the ranges)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (c0 == c1) return;                       // no blocks, or one range wrote the result itself
@@ -1148,19 +1162,16 @@ attention_join_kernel(const __grid_constant__ TcParams p) {
         const uint32_t member = offset + r, node = member % p.a.rows;
         const uint32_t head = kv_head * p.a.group + member / p.a.rows;
         if (node >= e.nodes) continue;
-        // (the row set began in range c0, behind its first block or at it: the second partial; the
-        // others began with it)
-        auto slot = [&](uint32_t c) {
-            return p.partial + (static_cast<uint64_t>(c) * 2 + (c == c0 ? 1u : 0u)) * p.slot_floats;
-        };
+        auto slot = [&](uint32_t which) { return p.partial + which * p.slot_floats; };
+        uint32_t ready = first_ready;           // every lane one of 32 ranges
         // The first ranges' values are asked for before anything else: all waits run together.
         constexpr uint32_t kAhead = 8;
-        const uint32_t ranges = c1 - c0 + 1;
         float v[kAhead][kMaxWidth / 32];
         auto ask = [&](uint32_t from) {
 #pragma unroll
             for (uint32_t i = 0; i < kAhead; ++i) {
-                const float* at = slot(c0 + min(from + i, ranges - 1)) + static_cast<uint64_t>(r) * width;
+                const uint32_t which = __shfl_sync(0xffffffffu, ready, min(from + i, ranges - 1) & 31u);
+                const float* at = slot(which) + static_cast<uint64_t>(r) * width;
 #pragma unroll
                 for (uint32_t k = 0; k < kMaxWidth / 32; ++k) v[i][k] = lane + 32 * k < width ? at[lane + 32 * k] : 0.0f;
             }
@@ -1168,7 +1179,7 @@ attention_join_kernel(const __grid_constant__ TcParams p) {
         ask(0);
         float top = __int_as_float(0xFF800000);
         for (uint32_t c = lane; c < ranges; c += 32) {
-            const float* at = slot(c0 + c);
+            const float* at = slot(c == lane ? ready : partial(c));
             const float part = at[static_cast<uint64_t>(p.row_cap) * (width + 1) + r];
             const float high = at[static_cast<uint64_t>(p.row_cap) * width + r];
             if (part != 0.0f) top = fmaxf(top, high);
@@ -1177,9 +1188,10 @@ attention_join_kernel(const __grid_constant__ TcParams p) {
         float sum = 0.0f, o[kMaxWidth / 32] = {};
         for (uint32_t base = 0; base < ranges; base += 32) {
             // Every lane has one range's factor ready; all lanes then add the ranges up in order.
+            if (base != 0) ready = partial(min(base + lane, ranges - 1));
             float factor = 0.0f, part = 0.0f;
             if (base + lane < ranges) {
-                const float* at = slot(c0 + base + lane);
+                const float* at = slot(ready);
                 part = at[static_cast<uint64_t>(p.row_cap) * (width + 1) + r];
                 const float high = at[static_cast<uint64_t>(p.row_cap) * width + r];
                 if (part != 0.0f) factor = exp2_fast((high - top) * p.scale_log2);
