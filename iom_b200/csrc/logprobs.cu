@@ -163,6 +163,10 @@ __device__ __forceinline__ uint64_t score_pair(float lo, float hi) {
 struct RunningSum {
     float m, z, t;
 };
+// How far a sum is moved to a new maximum. Beyond 10^4 its weights are zero all the same, and z times
+// the distance stays finite: logits may lie at the end of binary32 (masks of the leaf's lowest value),
+// and an infinite product would turn NaN under the weight of zero.
+__device__ __forceinline__ float score_step(float from, float to) { return fmaxf(from - to, -1e4f); }
 __device__ __forceinline__ RunningSum join_sums(const RunningSum& a, const RunningSum& b) {
     const float kNone = __int_as_float(0xFF800000);
     RunningSum r{fmaxf(a.m, b.m), 0.0f, 0.0f};
@@ -173,7 +177,7 @@ __device__ __forceinline__ RunningSum join_sums(const RunningSum& a, const Runni
         if (s.m == kNone) {
             z += s.z;
         } else {
-            const float d = s.m - r.m, f = score_exp2(d * kLog2e);
+            const float d = score_step(s.m, r.m), f = score_exp2(d * kLog2e);
             z = __fmaf_rn(s.z, f, z);
             t = __fmaf_rn(__fmaf_rn(s.z, d, s.t), f, t);
         }
@@ -306,7 +310,7 @@ score_kernel(const __grid_constant__ ScoreParams p) {
             if (high > m) {
                 if (m != kNone) {
                     // exp(x - high) = exp(x - m) f and (x - high) = (x - m) + d
-                    const float d = m - high, f = score_exp2(d * kLog2e);
+                    const float d = score_step(m, high), f = score_exp2(d * kLog2e);
                     const uint64_t f2 = score_pair(f, f), d2 = score_pair(d, d);
                     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(t2) : "l"(z2), "l"(d2));
                     asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(t2) : "l"(f2));
