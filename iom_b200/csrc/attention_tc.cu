@@ -1177,12 +1177,17 @@ attention_join_kernel(const __grid_constant__ TcParams p) {
             }
         };
         ask(0);
-        float top = __int_as_float(0xFF800000);
+        // A row is also bad when a score was seen and yet no weight was left (a score so large that its
+        // product with log2(e) overflowed): that range may hold all of the row's weight.
+        const float kNone = __int_as_float(0xFF800000);
+        float top = kNone;
+        bool bad = false;
         for (uint32_t c = lane; c < ranges; c += 32) {
             const float* at = slot(c == lane ? ready : partial(c));
             const float part = at[static_cast<uint64_t>(p.row_cap) * (width + 1) + r];
             const float high = at[static_cast<uint64_t>(p.row_cap) * width + r];
-            if (part != 0.0f) top = fmaxf(top, high);
+            top = fmaxf(top, high);             // (-inf: nothing seen in that range, or only scores of -inf)
+            bad = bad || (part == 0.0f && high != kNone);
         }
         for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
         float sum = 0.0f, o[kMaxWidth / 32] = {};
@@ -1194,7 +1199,7 @@ attention_join_kernel(const __grid_constant__ TcParams p) {
                 const float* at = slot(ready);
                 part = at[static_cast<uint64_t>(p.row_cap) * (width + 1) + r];
                 const float high = at[static_cast<uint64_t>(p.row_cap) * width + r];
-                if (part != 0.0f) factor = exp2_fast((high - top) * p.scale_log2);
+                if (high != kNone) factor = exp2_fast((high - top) * p.scale_log2);
             }
             const uint32_t count = min(32u, ranges - base);
             for (uint32_t i0 = 0; i0 < count; i0 += kAhead) {
@@ -1203,7 +1208,9 @@ attention_join_kernel(const __grid_constant__ TcParams p) {
                 for (uint32_t i = 0; i < kAhead; ++i) {
                     const float f = __shfl_sync(0xffffffffu, factor, (i0 + i) & 31u);
                     const float l = __shfl_sync(0xffffffffu, part, (i0 + i) & 31u);
-                    if (i0 + i >= count || l == 0.0f) continue;     // nothing seen in that range
+                    if (i0 + i >= count) continue;
+                    // (nothing seen in that range: zeros, or NaN from infinite values under weights of zero,
+                    // which may be those of visible tokens)
                     sum = __fmaf_rn(l, f, sum);
 #pragma unroll
                     for (uint32_t k = 0; k < kMaxWidth / 32; ++k) o[k] = __fmaf_rn(v[i][k], f, o[k]);
@@ -1211,7 +1218,7 @@ attention_join_kernel(const __grid_constant__ TcParams p) {
             }
         }
         const float inverse = 1.0f / sum;
-        bool bad = !(sum > 0.0f && sum <= 3.0e38f);
+        bad = bad || !(sum > 0.0f && sum <= 3.0e38f);
 #pragma unroll
         for (uint32_t k = 0; k < kMaxWidth / 32; ++k) {
             o[k] *= inverse;
