@@ -691,7 +691,9 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             }
 
             const float kNone = __int_as_float(0xFF800000);
-            float top = kNone, sum = 0.0f;                      // running maximum (of S) and sum
+            // Running maximum (of S), minus it scaled, and sum. Maxima are compared scaled: the difference of
+            // two scores may overflow where that of the scaled ones does not.
+            float top = kNone, shift = 0.0f, sum = 0.0f;
             const uint32_t first = piece.first_token;
             // Tokens from here on may be hidden from some row of the tile.
             const uint32_t clear = TREE ? start : piece.row0 + x * p.tile_rows + 1;
@@ -748,10 +750,11 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                     const float high = fmaxf(top, fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])));
                     // The first tokens seen, or a maximum that grew beyond what P may: a new reference.
                     const bool fresh = top == kNone;
-                    const bool grow = !fresh && (high - top) * p.scale_log2 > kRescale;
+                    const float reach = high * p.scale_log2, rise = reach + shift;
+                    const bool grow = !fresh && rise > kRescale;
                     if (__any_sync(0xffffffffu, grow)) {
                         // (not the first step; these scores came behind the products of the steps before)
-                        const float factor = grow ? exp2_fast((top - high) * p.scale_log2) : 1.0f;
+                        const float factor = grow ? exp2_fast(-rise) : 1.0f;
                         sum *= factor;
                         for (uint32_t c = 0; c < slices; ++c) {
                             uint32_t o[16];
@@ -762,8 +765,10 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                             tmem_store16(o_at + c * 16, o);
                         }
                     }
-                    if (fresh || grow) top = high;
-                    const float shift = top == kNone ? 0.0f : -(top * p.scale_log2);
+                    if (fresh || grow) {
+                        top = high;
+                        shift = high == kNone ? 0.0f : -reach;
+                    }
                     const uint64_t shift2 = pair(shift, shift);
                     uint64_t sums[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -1199,7 +1204,7 @@ attention_join_kernel(const __grid_constant__ TcParams p) {
                 const float* at = slot(ready);
                 part = at[static_cast<uint64_t>(p.row_cap) * (width + 1) + r];
                 const float high = at[static_cast<uint64_t>(p.row_cap) * width + r];
-                if (high != kNone) factor = exp2_fast((high - top) * p.scale_log2);
+                if (high != kNone) factor = exp2_fast(high * p.scale_log2 - top * p.scale_log2);
             }
             const uint32_t count = min(32u, ranges - base);
             for (uint32_t i0 = 0; i0 < count; i0 += kAhead) {
