@@ -392,7 +392,8 @@ int iomb_sdpa_canonicalize_output(const iomb_view* out, void* stream);
  * may be none. Rows outside every sequence are neither read nor written. `status` (device
  * word) becomes 0, or 1 when the offsets descend or pass T: then nothing is written.
  * Scores, the softmax's maximum and sum and the weighted sum are binary32; the weights are
- * rounded to the leaf once, before they meet v, and the result once, when it is stored. Special rows as in
+ * rounded to the leaf once, before they meet v (an F16 weight is off by half a step, or by 2^-32 of the
+ * row's largest where that is more), and the result once, when it is stored. Special rows as in
  * iomb_sdpa_softmax: a NaN among a row's scores, or only -inf, makes the row the quiet NaN,
  * +inf scores share the weight; stored -0 and NaN are canonical. What masked places hold has
  * no influence. D up to 256; multiples of 16 up to 128 run on the tensor cores. `scale` is positive and

@@ -61,6 +61,7 @@ __device__ __forceinline__ unsigned char* attn_out_piece(const AttnOperand& o, u
 
 struct LeafBf16 {
     static constexpr uint32_t kFormat = 1;      // operand format of the matrix instructions
+    static constexpr float kWeightLog = 0.0f;   // log2 of the weight that a row's maximum gets in them
     static __device__ __forceinline__ float decode(uint16_t code) {
         return __uint_as_float(static_cast<uint32_t>(code) << 16);
     }
@@ -77,6 +78,7 @@ struct LeafBf16 {
 };
 struct LeafF16 {
     static constexpr uint32_t kFormat = 0;
+    static constexpr float kWeightLog = 7.0f;
     static __device__ __forceinline__ float decode(uint16_t code) {
         return __half2float(__ushort_as_half(code));
     }

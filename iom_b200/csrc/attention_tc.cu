@@ -8,7 +8,9 @@
 //   O += P V           tcgen05.mma, P from tensor memory, V from shared memory, O in tensor memory
 // with the running maximum m and sum l of each row in its thread. O is rescaled only when a
 // row's maximum grows by more than 2^8 (P then stays below 2^8, far from any overflow); the sum
-// takes the unrounded exponentials. While one tile's softmax runs, the other tile's products do.
+// takes the unrounded exponentials. F16 holds P times 2^7 (below 2^15), so that weights down to 2^-32 of
+// the maximum's count: times one, those below 2^-25 vanished beside the sum that held them, 1 part in
+// 1000 where 60000 of them stood against one large weight. While one tile's softmax runs, the other tile's products do.
 // P is handed over in two halves, so that its product with V begins while the second half's
 // exponentials are still computed.
 //
@@ -691,8 +693,8 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             }
 
             const float kNone = __int_as_float(0xFF800000);
-            // Running maximum (of S), minus it scaled, and sum. Maxima are compared scaled: the difference of
-            // two scores may overflow where that of the scaled ones does not.
+            // Running maximum (of S), what is added to scaled scores, and sum. Maxima are compared scaled: the
+            // difference of two scores may overflow where that of the scaled ones does not.
             float top = kNone, shift = 0.0f, sum = 0.0f;
             const uint32_t first = piece.first_token;
             // Tokens from here on may be hidden from some row of the tile.
@@ -750,7 +752,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                     const float high = fmaxf(top, fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])));
                     // The first tokens seen, or a maximum that grew beyond what P may: a new reference.
                     const bool fresh = top == kNone;
-                    const float reach = high * p.scale_log2, rise = reach + shift;
+                    const float next = Leaf::kWeightLog - high * p.scale_log2, rise = shift - next;
                     const bool grow = !fresh && rise > kRescale;
                     if (__any_sync(0xffffffffu, grow)) {
                         // (not the first step; these scores came behind the products of the steps before)
@@ -767,7 +769,7 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
                     }
                     if (fresh || grow) {
                         top = high;
-                        shift = high == kNone ? 0.0f : -reach;
+                        shift = high == kNone ? 0.0f : next;
                     }
                     const uint64_t shift2 = pair(shift, shift);
                     uint64_t sums[4] = {0, 0, 0, 0};
@@ -1204,7 +1206,8 @@ attention_join_kernel(const __grid_constant__ TcParams p) {
                 const float* at = slot(ready);
                 part = at[static_cast<uint64_t>(p.row_cap) * (width + 1) + r];
                 const float high = at[static_cast<uint64_t>(p.row_cap) * width + r];
-                if (high != kNone) factor = exp2_fast(high * p.scale_log2 - top * p.scale_log2);
+                // (each range's weights were taken against its maximum as rounded here)
+                if (high != kNone) factor = exp2_fast((Leaf::kWeightLog - top * p.scale_log2) - (Leaf::kWeightLog - high * p.scale_log2));
             }
             const uint32_t count = min(32u, ranges - base);
             for (uint32_t i0 = 0; i0 < count; i0 += kAhead) {
