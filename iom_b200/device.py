@@ -1048,18 +1048,21 @@ class B200Queue:
     # Small index arrays are device addresses of uint32 words (int32 for parents), as in
     # cache_append_batched; `status` is a device word that becomes 0, or 1 when the arrays'
     # values do not fit. They are read when the operation runs.
-    def _operands(self, what: str, *views):
-        """The ABI snapshots of an operation's views (None stays None)."""
+    def _operands(self, what: str, views, optional=()):
+        """The ABI snapshots and the owners of an operation's views; an optional one may be None."""
         device = self._device
-        references = []
-        for view in views:
+        references, owners = [], []
+        for place, view in enumerate((*views, *optional)):
             if view is None:
+                if place < len(views):
+                    raise ValueError(f"{what} requires all of its operands")
                 references.append(None)
                 continue
             if getattr(view.owner, "device", None) is not device:
                 self._check_view(view, what)
             references.append(view.abi_reference())
-        return references
+            owners.append(view.owner)
+        return references, owners
 
     def sdpa_packed(self, q: TensorView, k: TensorView, v: TensorView, out: TensorView,
                     offsets: int, sequences: int, status: int, scale: Optional[float] = None) -> int:
@@ -1067,7 +1070,7 @@ class B200Queue:
         out [T, Hq*D], BF16 or F16; `offsets` holds sequences + 1 ascending row borders. `scale`
         None is 1/sqrt(D). See iomb_sdpa_packed."""
         try:
-            a, b, c, d = self._operands("sdpa_packed", q, k, v, out)
+            (a, b, c, d), owners = self._operands("sdpa_packed", (q, k, v, out))
             if not 0 <= sequences < 1 << 32:
                 raise ValueError("sdpa_packed: the number of sequences is out of range")
             if scale is None:
@@ -1075,11 +1078,10 @@ class B200Queue:
         except BaseException as error:
             return _exception_to_oid(error)
         return self._submit(
-            lambda stream: self._lib.iomb_sdpa_packed(a, b, c, d, offsets, sequences, scale, status, stream),
-            (q.owner, k.owner, v.owner, out.owner))
+            lambda stream: self._lib.iomb_sdpa_packed(a, b, c, d, offsets, sequences, scale, status, stream), owners)
 
     def sdpa_tree_workspace_requirements(self, q: TensorView, k: TensorView) -> WorkspaceRequirements:
-        a, b = self._operands("sdpa_tree", q, k)
+        (a, b), _ = self._operands("sdpa_tree", (q, k))
         nbytes = ctypes.c_uint64()
         status = self._lib.iomb_sdpa_tree_workspace_bytes(a, b, ctypes.byref(nbytes))
         if status != 0:
@@ -1093,12 +1095,13 @@ class B200Queue:
         the single-token decode. q [B, Hq, N, D], k and v [B, Hkv, C, D], out [B, N, Hq*D];
         `parents` 0 makes every tree a chain, `counts` 0 means N nodes each. See iomb_sdpa_tree."""
         try:
-            a, b, c, d = self._operands("sdpa_tree", q, k, v, out)
-            address, nbytes, owner = 0, 0, None
+            (a, b, c, d), owners = self._operands("sdpa_tree", (q, k, v, out))
+            address, nbytes = 0, 0
             if workspace is not None and not workspace.empty():
                 if not self._device.owns_workspace(workspace.owner):
                     raise ValueError("sdpa_tree requires a live workspace of this device")
-                address, nbytes, owner = workspace.address(), workspace.byte_size(), workspace.owner
+                address, nbytes = workspace.address(), workspace.byte_size()
+                owners.append(workspace.owner)
             if scale is None:
                 scale = q.spec.shape[-1] ** -0.5
         except BaseException as error:
@@ -1106,7 +1109,7 @@ class B200Queue:
         return self._submit(
             lambda stream: self._lib.iomb_sdpa_tree(a, b, c, d, lengths, parents or None, counts or None, scale,
                                                     address, nbytes, status, stream),
-            (q.owner, k.owner, v.owner, out.owner, owner))
+            owners)
 
     def cache_compact(self, k: TensorView, v: Optional[TensorView], lengths: int, accepted: int,
                       width: int, counts: int, status: int) -> int:
@@ -1114,14 +1117,14 @@ class B200Queue:
         place, in caches [B, ..., C, D]; `accepted` is [B, width], ascending. See
         iomb_cache_compact."""
         try:
-            a, b = self._operands("cache_compact", k, v)
+            (a, b), owners = self._operands("cache_compact", (k,), (v,))
             if not 0 <= width < 1 << 32:
                 raise ValueError("cache_compact: width is out of range")
         except BaseException as error:
             return _exception_to_oid(error)
         return self._submit(
             lambda stream: self._lib.iomb_cache_compact(a, b, lengths, accepted, width, counts, status, stream),
-            (k.owner, None if v is None else v.owner))
+            owners)
 
     def token_logprobs(self, logits: TensorView, tokens: TensorView, logprob: TensorView,
                        entropy: Optional[TensorView], status: int,
@@ -1131,10 +1134,9 @@ class B200Queue:
         tokens. logits [..., R, V], tokens, logprob and entropy [..., 1, R], top_* [..., R, K].
         See iomb_token_logprobs."""
         try:
-            views = (logits, tokens, logprob, entropy, top_logprobs, top_tokens)
-            a, b, c, d, e, f = self._operands("token_logprobs", *views)
+            (a, b, c, d, e, f), owners = self._operands("token_logprobs", (logits, tokens, logprob),
+                                                        (entropy, top_logprobs, top_tokens))
         except BaseException as error:
             return _exception_to_oid(error)
         return self._submit(
-            lambda stream: self._lib.iomb_token_logprobs(a, b, c, d, e, f, status, stream),
-            tuple(view.owner for view in views if view is not None))
+            lambda stream: self._lib.iomb_token_logprobs(a, b, c, d, e, f, status, stream), owners)
