@@ -577,32 +577,46 @@ extern "C" int iomb_cache_compact(const iomb_view* k, const iomb_view* v, const 
         bool same = k->rank == v->rank && k->dtype == v->dtype;
         for (uint32_t i = 0; i < k->rank && same; ++i) same = k->dims[i] == v->dims[i];
         if (!same) return fail(IOMB_ERR_INVALID_ARGUMENT, "cache_compact: k and v shapes or encodings differ");
-        if (storage_overlaps(*k, fk, *v, fv)) {
-            return fail(IOMB_ERR_INVALID_ARGUMENT, "cache_compact: k and v storage overlap");
-        }
     }
-    for (const iomb_view* view : {k, v}) {
-        // Rows move in place, so two indices must not name one plane.
-        if (view == nullptr) continue;
-        uint64_t pairs[kMaxLead][2];
+    // Rows move in place, so two indices must not name one plane. Axes as (stride, extent), by stride:
+    // distinct where every stride passes all that the smaller ones reach.
+    auto distinct = [](const iomb_view& view, uint64_t second) {
+        uint64_t pairs[kMaxLead + 1][2];
         uint32_t n = 0;
-        for (uint32_t axis = 0; axis + 2 < view->rank; ++axis) {
-            if (view->dims[axis] == 1) continue;
+        for (uint32_t axis = 0; axis + 1 < view.rank; ++axis) {
+            // (the last one: `second` planes on lies the first plane of the other cache)
+            const bool other = axis + 2 == view.rank;
+            const uint64_t stride = other ? second : view.plane_strides[axis], extent = other ? 2 : view.dims[axis];
+            if (other ? second == 0 : extent == 1) continue;
             uint32_t at = n++;
-            while (at > 0 && pairs[at - 1][0] > view->plane_strides[axis]) {
+            while (at > 0 && pairs[at - 1][0] > stride) {
                 pairs[at][0] = pairs[at - 1][0];
                 pairs[at][1] = pairs[at - 1][1];
                 --at;
             }
-            pairs[at][0] = view->plane_strides[axis];
-            pairs[at][1] = view->dims[axis];
+            pairs[at][0] = stride;
+            pairs[at][1] = extent;
         }
         uint64_t reach = 0;     // furthest plane the axes with smaller strides get to
         for (uint32_t i = 0; i < n; ++i) {
-            if (pairs[i][0] <= reach) {
-                return fail(IOMB_ERR_INVALID_ARGUMENT, "cache_compact: planes of the cache overlap");
-            }
+            if (pairs[i][0] <= reach) return false;
             reach += pairs[i][0] * (pairs[i][1] - 1);
+        }
+        return true;
+    };
+    if (!distinct(*k, 0) || (v != nullptr && !distinct(*v, 0))) {
+        return fail(IOMB_ERR_INVALID_ARGUMENT, "cache_compact: planes of the cache overlap");
+    }
+    if (v != nullptr && storage_overlaps(*k, fk, *v, fv)) {
+        // Keys and values that alternate inside one owner are a cache with one more axis of two.
+        bool alternate = k->base == v->base && k->plane_offset != v->plane_offset;
+        for (uint32_t axis = 0; axis + 2 < k->rank; ++axis) {
+            alternate = alternate && (k->dims[axis] == 1 || k->plane_strides[axis] == v->plane_strides[axis]);
+        }
+        const uint64_t apart = k->plane_offset > v->plane_offset ? k->plane_offset - v->plane_offset
+                                                                 : v->plane_offset - k->plane_offset;
+        if (!alternate || !distinct(*k, apart)) {
+            return fail(IOMB_ERR_INVALID_ARGUMENT, "cache_compact: k and v storage overlap");
         }
     }
     for (const void* address : {static_cast<const void*>(lengths), static_cast<const void*>(accepted),
