@@ -390,7 +390,8 @@ int iomb_sdpa_canonicalize_output(const iomb_view* out, void* stream);
  * iomb_sdpa_canonicalize_output), one leaf: BF16 or F16. `offsets` is a device array of
  * sequences + 1 ascending rows; sequence s holds the rows offsets[s] .. offsets[s+1]-1, which
  * may be none. Rows outside every sequence are neither read nor written. `status` (device
- * word) becomes 0, or 1 when the offsets descend or pass T: then nothing is written.
+ * word) becomes 0, or 1 when the offsets descend or pass T: then nothing is written (2: a wait inside
+ * the kernel gave up, see iomb_sdpa_wait_timeouts).
  * Scores, the softmax's maximum and sum and the weighted sum are binary32; the weights are
  * rounded to the leaf once, before they meet v (an F16 weight is off by half a step, or by 2^-32 of the
  * row's largest where that is more), and the result once, when it is stored. Special rows as in
@@ -415,7 +416,7 @@ int iomb_sdpa_packed(const iomb_view* q, const iomb_view* k, const iomb_view* v,
  * the rows before the tree, its ancestors and itself. N = 1 is the single-token decode. Output
  * rows at or beyond counts[b] keep their bytes. `status` becomes 0, or 1 when a sequence does
  * not fit (lengths[b] + counts[b] > C or counts[b] > N: it is skipped) or a parent does not
- * lie before its node or is below -1 (the node then counts as a root).
+ * lie before its node or is below -1 (the node then counts as a root), or 2 as in iomb_sdpa_packed.
  * `workspace` holds iomb_sdpa_tree_workspace_bytes bytes of device memory, 32-byte aligned:
  * long caches are cut into ranges whose partial sums meet there. Its contents need no set-up
  * and mean nothing after the call; two calls that may overlap on the GPU use two workspaces.

@@ -53,7 +53,10 @@ tree_rows_kernel(const AttnParams p) {
         const int32_t* parents = p.parents != nullptr ? p.parents + static_cast<uint64_t>(b) * p.rows : nullptr;
         attend_row<Leaf>(p, b, h, node, TreeRow{e.length, node, parents});
     }
-    if (warp == 0) warp_report_tree(p);
+    if (warp == 0) {
+        const bool bad = warp_tree_bad(p);
+        if ((threadIdx.x & 31u) == 0) *p.status = bad ? 1u : 0u;
+    }
 }
 
 // ---- admission ----------------------------------------------------------------------------------

@@ -265,8 +265,8 @@ __device__ __forceinline__ bool warp_borders_ok(const AttnParams& p) {
     return __all_sync(0xffffffffu, ok);
 }
 
-// One warp reports a tree call's arguments: extents that do not fit, parents not before their nodes.
-__device__ __forceinline__ void warp_report_tree(const AttnParams& p) {
+// One warp looks through a tree call's arguments: extents that do not fit, parents not before their nodes.
+__device__ __forceinline__ bool warp_tree_bad(const AttnParams& p) {
     bool bad = false;
     const uint32_t lane = threadIdx.x & 31u;
     for (uint32_t b = lane; b < p.batch; b += 32) bad = bad || tree_extent(p, b).bad;
@@ -279,8 +279,7 @@ __device__ __forceinline__ void warp_report_tree(const AttnParams& p) {
             bad = bad || (node < nodes && (parent >= static_cast<int32_t>(node) || parent < -1));
         }
     }
-    bad = __any_sync(0xffffffffu, bad);
-    if (lane == 0) *p.status = bad ? 1u : 0u;
+    return __any_sync(0xffffffffu, bad);
 }
 
 // The tensor-core kernel (attention_tc.cu). The workspace is the partial sums of a tree call.

@@ -51,7 +51,7 @@
 // workers 8 and 9 issue A's and B's matrix instructions, 10 and 11 their copies and queries. The
 // last four hand registers to the softmax (2 x 128 x 208 + 128 x 80 of the 384 x 168 a CTA starts
 // with).
-// Every wait is bounded; one that gives up ends all roles and is counted.
+// Every wait is bounded; one that gives up ends all roles, is counted and makes the status 2.
 #include <cuda.h>
 
 #include <stdio.h>
@@ -559,6 +559,9 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
             bar_init(&sh.landed[x], 1);
         }
         sh.stop = 0;
+        // The status begins at zero and only grows: 1 from this CTA's check of the arguments, 2 from a CTA
+        // in which a wait gave up (a second after its start at the least, and the first CTA starts first).
+        if (TREE && blockIdx.x == 0) *p.a.status = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     tmem_before_sync();
@@ -1091,14 +1094,20 @@ attention_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ 
     }
     if constexpr (TREE) {
         // (behind the copies, beside the last products)
-        if (warp == 9 && blockIdx.x == 0) warp_report_tree(p.a);
+        if (warp == 9 && blockIdx.x == 0) {
+            const bool bad = warp_tree_bad(p.a);
+            if (bad && lane == 0) atomicMax(p.a.status, 1u);
+        }
     }
     tmem_before_sync();
     __syncthreads();
     tmem_after_sync();
     if (warp == 8) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns));
-        if (lane == 0 && sh.stop != 0) atomicAdd(&g_attention_timeouts, 1u);
+        if (lane == 0 && sh.stop != 0) {
+            atomicAdd(&g_attention_timeouts, 1u);
+            atomicMax(p.a.status, 2u);
+        }
     }
 }
 
