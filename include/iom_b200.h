@@ -396,7 +396,8 @@ int iomb_sdpa_canonicalize_output(const iomb_view* out, void* stream);
  * rounded to the leaf once, before they meet v (an F16 weight is off by half a step, or by 2^-32 of the
  * row's largest where that is more), and the result once, when it is stored. Special rows as in
  * iomb_sdpa_softmax: a NaN among a row's scores, or only -inf, makes the row the quiet NaN,
- * +inf scores share the weight; stored -0 and NaN are canonical. What masked places hold has
+ * +inf scores share the weight; stored -0 and NaN are canonical. A weight that underflows is zero,
+ * and zero times an infinite value of a visible row is NaN. What masked places hold has
  * no influence. D up to 256; multiples of 16 up to 128 run on the tensor cores. `scale` is positive and
  * finite (1/sqrtf(D) usually). The output overlaps no input.
  * No counterpart in the reference, whose sdpa takes one sequence (the caller's loop over
@@ -428,7 +429,7 @@ int iomb_sdpa_tree(const iomb_view* q, const iomb_view* k, const iomb_view* v, c
                    void* workspace, uint64_t workspace_bytes, uint32_t* status, void* stream);
 
 /* iomb_rmsnorm_copy_timeouts for the attention kernels: CTAs in which a bounded wait gave up
- * (never expected: their results are incomplete). Synchronous. */
+ * (never expected: their results are incomplete, and the call's status is 2). Synchronous. */
 int iomb_sdpa_wait_timeouts(unsigned int* count);
 
 /*
@@ -438,7 +439,8 @@ int iomb_sdpa_wait_timeouts(unsigned int* count);
  * array `accepted` is [B, width]; a sequence's path ascends strictly below width, as a walk
  * from a root does. No other row changes. `status` becomes 0, or 1 when some path does not
  * ascend, reaches width or the end of the cache, or counts[b] > width: that b is skipped.
- * Byte-multiple leaves. The planes of a view are distinct, and k and v do not overlap.
+ * Byte-multiple leaves. The planes of a view are distinct, and k and v have none in common (views of
+ * one owner may alternate, as in [B, 2, H, C, D]).
  * No counterpart in the reference.
  */
 int iomb_cache_compact(const iomb_view* k, const iomb_view* v, const uint32_t* lengths,

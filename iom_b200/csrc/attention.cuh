@@ -266,6 +266,9 @@ __device__ __forceinline__ bool warp_borders_ok(const AttnParams& p) {
 }
 
 // One warp looks through a tree call's arguments: extents that do not fit, parents not before their nodes.
+// (One element a lane and round, so many large trees over short caches wait for it: 64 of 256 nodes, 32
+// heads on 8, D 64, caches of 456 take 466 us with parents and 174 as chains; 8 of 64 nodes over caches of
+// 8192 57 and 55.)
 __device__ __forceinline__ bool warp_tree_bad(const AttnParams& p) {
     bool bad = false;
     const uint32_t lane = threadIdx.x & 31u;

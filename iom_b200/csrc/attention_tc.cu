@@ -39,11 +39,11 @@
 // values beside the sequence in its first and last tile are zeroed as they arrive.
 //
 // What bounds it (one B200; rates by the algorithm's bytes and products):
-//   packed 4 x 4096 rows   32 heads on 4, D 128: 520 us, 1060 TFLOP/s. Per step of 128 x 128 scores the
+//   packed 8192 rows       32 heads on 8, D 128: 508 us, 1080 TFLOP/s. Per step of 128 x 128 scores the
 //                          exponentials take 1024 clocks of the SM's special-function units, the two
 //                          products 1024 of the tensor cores, and neither reaches beyond 53 % of the
 //                          time: what is left is the softmax's other instructions between two handovers.
-//   tree, long caches      8 trees, 427 MB of keys and values: 90 us, 4.7 TB/s
+//   tree, long caches      2 trees of 5 nodes, caches of 100001 rows (427 MB): 88 us, 4.9 TB/s
 //   tree, single tokens    64 decodes: 28 us, 2.4 TB/s; the changes between row sets and the second kernel
 //
 // Warps: 0-3 softmax of A, 4-7 softmax of B, 8 issues the matrix instructions, 9 the copies, 10

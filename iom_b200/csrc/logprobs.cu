@@ -16,8 +16,11 @@
 // to the row's owner, which joins them. The best tokens take no second pass: of the maxima of G
 // disjoint groups of columns at least K reach the K-th largest, tau, so every one of the K best
 // reaches it too, and only the slots whose own maximum does (about K of them) are read again for
-// their elements. The owner ranks these candidates. Rows where that breaks down (more than 256
-// candidates, which takes ties by the hundred, or NaN) are ranked by one warp that walks the row.
+// their elements. The owner ranks these candidates. Rows where that breaks down are
+// ranked by one warp that walks the row: with NaN, or with more than 256 candidates. tau has 16 leading
+// bits, so those are values by the hundred that tie or lie within one part in 128 of the K-th best, or
+// fewer than K tokens beside a finite mask. It costs about 160 us a walk of 32000 columns (64 rows of F32
+// 11 us, 161 with one such row and 185 with 64; 2045 rows of 50021 92 us, 1117 when all are such).
 //
 // Bound by HBM where there are many rows: 2045 rows of 50021 F32 logits take 73 us per call on a B200
 // (5.6 TB/s). 64 rows of 32000 BF16 take 9.3 us, bound by the chain load, cluster
