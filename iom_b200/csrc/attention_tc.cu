@@ -9,8 +9,9 @@
 // with the running maximum m and sum l of each row in its thread. O is rescaled only when a
 // row's maximum grows by more than 2^8 (P then stays below 2^8, far from any overflow); the sum
 // takes the unrounded exponentials. F16 holds P times 2^7 (below 2^15), so that weights down to 2^-32 of
-// the maximum's count: times one, those below 2^-25 vanished beside the sum that held them, 1 part in
-// 1000 where 60000 of them stood against one large weight. While one tile's softmax runs, the other tile's products do.
+// the maximum's count: times one, those below 2^-25 vanished beside the sum that held them (60000 weights
+// of 2^-26.5 against one large weight are 6e-4 of the result). While one tile's softmax runs, the other
+// tile's products do.
 // P is handed over in two halves, so that its product with V begins while the second half's
 // exponentials are still computed.
 //
